@@ -28,7 +28,7 @@ own = False
 DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 SIZE = {"bf16": 2, "f16": 2, "f32": 4}
 LEVELS = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
-# scale bytes that leave every code a finite and exact value of the type
+# scale bytes that leave every code a finite and exact value of the type; a byte above reads as the last
 BYTES = {"bf16": (2, 252), "f16": (104, 140), "f32": (2, 252)}
 
 
@@ -171,11 +171,11 @@ def _quantise(x, dtype):
 
 def _values(codes, scales, dtype):
     """The values, float32 [..., D], that codes [..., D / 2] and scale bytes [..., D / 32] stand for."""
-    lo, hi = BYTES[dtype]
+    hi = BYTES[dtype][1]
     table = torch.tensor(LEVELS + [-v for v in LEVELS], device=codes.device)
     nib = torch.stack([codes & 15, codes >> 4], -1).flatten(-2)
     nib = nib.unflatten(-1, (4, -1, 8)).transpose(-3, -2).flatten(-3).int()
-    scale = (scales.int().clamp(lo, hi) << 23).view(torch.float32)
+    scale = (scales.int().clamp(max=hi) << 23).view(torch.float32)
     return (table[nib].unflatten(-1, (-1, 32)) * scale.unsqueeze(-1)).flatten(-2)
 
 
@@ -396,7 +396,7 @@ def _nearest(x, dtype):
 
 def _decode(codes, scales, dtype):
     """float64 values of cache rows, element by element of the byte layout."""
-    lo, hi = BYTES[dtype]
+    hi = BYTES[dtype][1]
     d = codes.shape[-1] * 2
     e = torch.arange(d, device=codes.device)
     chunk, i = e // 8, e % 8
@@ -404,7 +404,7 @@ def _decode(codes, scales, dtype):
     code = (codes.int()[..., byte] >> (4 * (i % 2)).int()) & 15
     m = code & 7
     mag = torch.where(m < 2, 0.5 * m, (2 + (m & 1)) * torch.exp2((m >> 1).double() - 2))
-    power = torch.exp2(scales.double().clamp(lo, hi) - 127)
+    power = torch.exp2(scales.double().clamp(max=hi) - 127)
     return torch.where(code > 7, -mag, mag) * power.repeat_interleave(32, -1)
 
 
