@@ -52,7 +52,7 @@ const char* fxpr_error_string(int code);
 
 /* ABI revision of this header, and of the library: bumped when a signature
  * changes or the bindings need a new entry point. */
-#define FXPR_ABI_VERSION 4
+#define FXPR_ABI_VERSION 5
 int fxpr_abi_version(void);
 
 /*
@@ -387,6 +387,100 @@ int fxpr_reshape_and_cache(const void* key, const void* value, void* k_cache,
                            int64_t stride_kc_slot, int64_t stride_kc_head,
                            int64_t stride_vc_block, int64_t stride_vc_slot,
                            int64_t stride_vc_head, void* stream);
+
+/*
+ * The paged KV cache in 4 bits (mx4): 32 consecutive elements of a row (one
+ * token, one kv head, K or V) share a scale byte b, which stands for
+ * 2^(b - 127), and an element is a 4-bit code, sign and magnitude 0 .5 1 1.5 2
+ * 3 4 6 (E2M1). Two uint8 tensors [num_blocks, 2 (K, V), block_size,
+ * num_kv_heads, ...], codes with head_size / 2 and scales with head_size / 32
+ * bytes a row: 17 bytes for 32 elements. Byte order of a row's codes: the
+ * 8-element chunk c is the 4-byte unit (c % 4) * (head_size / 32) + c / 4,
+ * its element i in bits 4 i .. 4 i + 3 of the unit. A scale byte above the
+ * largest one of the type that is read (f16: 140, bf16 / f32: 252) reads as
+ * that one, so every byte pattern reads as finite values.
+ *
+ * head_size 64, 128 or 256. Strides of codes and scales in bytes, unit stride
+ * along a row; codes strides and address multiples of 16, scales ones of
+ * head_size / 32. (Rows of one head laid out page by page, heads before slots,
+ * are the fastest order for attention; any order works.)
+ */
+
+/*
+ * Quantising write: for each token t with slot = slot_mapping[t] in [0,
+ * num_blocks * block_size), key[t, h, :] and value[t, h, :] become rows of the
+ * cache; other slots (padding) are skipped. Per block, with amax its largest
+ * magnitude: b is the byte with amax / 2^(b - 127) in (3.5, 7], limited to
+ * [104, 140] for f16 and [2, 252] for bf16 / f32 inputs; a code is
+ * x / 2^(b - 127) rounded to the nearest magnitude (ties to the even code) and
+ * saturated at 6; NaN becomes 0, an infinity saturates. The slots of one call
+ * are distinct (a slot given twice holds parts of either row). key / value: f16
+ * / bf16 / f32 (dtype), 16-byte aligned rows, strides in elements.
+ * No counterpart in the reference, whose backend refuses a quantised cache
+ * (fxpr_vllm/attention_backend.py:40-277).
+ */
+int fxpr_reshape_and_cache_mx4(
+    const void* key, const void* value, void* codes, void* scales, int dtype,
+    const int64_t* slot_mapping, int64_t num_tokens, int num_kv_heads,
+    int head_size, int block_size, int64_t num_blocks, int64_t stride_key_token,
+    int64_t stride_key_head, int64_t stride_value_token,
+    int64_t stride_value_head, int64_t stride_codes_block,
+    int64_t stride_codes_half, int64_t stride_codes_slot,
+    int64_t stride_codes_head, int64_t stride_scales_block,
+    int64_t stride_scales_half, int64_t stride_scales_slot,
+    int64_t stride_scales_head, void* stream);
+
+/*
+ * Read back: key[i, h, :] and value[i, h, :] (contiguous [num_slots,
+ * num_kv_heads, head_size] of dtype f16 / bf16 / f32) = the values that the
+ * rows of slot slot_mapping[i] stand for, rounded to dtype (exact for rows
+ * written from that type); zeros for a slot outside the cache. No counterpart
+ * in the reference.
+ */
+int fxpr_gather_cache_mx4(
+    const void* codes, const void* scales, void* key, void* value, int dtype,
+    const int64_t* slot_mapping, int64_t num_slots, int num_kv_heads,
+    int head_size, int block_size, int64_t num_blocks,
+    int64_t stride_codes_block, int64_t stride_codes_half,
+    int64_t stride_codes_slot, int64_t stride_codes_head,
+    int64_t stride_scales_block, int64_t stride_scales_half,
+    int64_t stride_scales_slot, int64_t stride_scales_head, void* stream);
+
+/*
+ * fxpr_unified_attention over a cache in 4 bits: the same formula, metadata and
+ * bits as over a cache of io_dtype (f16 / bf16) that holds the values the codes
+ * stand for, so outputs are bitwise independent of the split count, of the
+ * batch and of max_query_len. page_size: a power of two, 16 or more. q rows
+ * 16-byte aligned. The launch needs a workspace of fxpr_attention_mx4_plan()
+ * bytes when that is non-zero (no zeroing). num_kv_splits: 0 = automatic. No
+ * counterpart in the reference.
+ */
+int fxpr_unified_attention_mx4(
+    const void* q, const void* codes, const void* scales, void* o, int io_dtype,
+    const int32_t* query_start_loc, const int32_t* seq_lens,
+    const int32_t* block_table, const float* alibi_slopes, int num_requests,
+    int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim,
+    int page_size, int max_query_len, int max_blocks_per_seq,
+    int64_t num_blocks, int64_t stride_q_token, int64_t stride_q_head,
+    int64_t stride_codes_block, int64_t stride_codes_half,
+    int64_t stride_codes_slot, int64_t stride_codes_head,
+    int64_t stride_scales_block, int64_t stride_scales_half,
+    int64_t stride_scales_slot, int64_t stride_scales_head,
+    int64_t stride_o_token, int64_t stride_o_head, int64_t stride_bt_row,
+    int is_causal, float softmax_scale_log2, float softcap_log2,
+    int window_size, int int_bits, int frac_bits, int num_kv_splits,
+    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes fxpr_unified_attention_mx4 needs for this launch (0 = none:
+ * also for arguments it rejects). plan: NULL or 4 ints that receive whether
+ * requests of 48 query rows per kv head or more run in 64-row workgroups, the
+ * key splits of those and of the 16-row workgroups, and the tokens per request
+ * that have records (0: every token). */
+int64_t fxpr_attention_mx4_plan(int num_requests, int64_t num_tokens,
+                                int num_heads, int num_kv_heads, int head_dim,
+                                int page_size, int max_query_len,
+                                int max_blocks_per_seq, int window_size,
+                                int int_bits, int num_kv_splits, int32_t* plan);
 
 #ifdef __cplusplus
 }

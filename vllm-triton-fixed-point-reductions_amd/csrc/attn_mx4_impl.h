@@ -1,0 +1,898 @@
+// Paged attention over the KV cache in 4 bits (format: mx4.h): prefill and
+// decode, the formula, chunk statistics and bits of attn_impl.h's kernels over
+// a cache of the values the codes stand for. Instantiated per activation type
+// in attn_mx4_{bf16,f16}.hip.
+//
+// Every code becomes an exact 16-bit float (one conversion per two elements,
+// the block's scale included) in the lane that feeds it to a matrix
+// instruction or writes it to LDS, so scores and weighted V are the 16-bit
+// MFMA chains of attn_impl.h in the same order. Scores are computed transposed
+// (keys as the MFMA's rows, query rows as its columns): lane (kg, row i =
+// lane % 16) gets keys 8 kg .. 8 kg + 7 of each 32-key step from two MFMAs
+// whose key rows are pi(i) = 8 (i / 4) + 4 h + i % 4, h = 0, 1, which is its
+// operand of the weighted-V MFMA: the weights never leave its registers.
+//
+// Two kernels:
+//   attn_mx4_rows16_kernel  16 query rows a workgroup (decode, short prompts).
+//     Bound by the cache's bytes, so its four waves take different key tiles of
+//     a chunk and share nothing but the chunk's maxima and integer sums.
+//   attn_mx4_rows64_kernel  64 query rows (prompts). Bound by vector
+//     arithmetic, so a key tile is unpacked once for the four waves.
+#pragma once
+
+#include "attn_impl.h"
+#include "mx4.h"
+
+namespace fxpr {
+namespace attn {
+namespace m4 {
+
+using mx4::u32x2;
+
+struct Mx4Args {
+  AttnArgs a;  // (k, v and their strides unused)
+  const uint8_t* kc;  // K codes, V codes, K scales, V scales
+  const uint8_t* vc;
+  const uint8_t* ks;
+  const uint8_t* vs;
+  uint32_t c_blk, c_slot, c_head, s_blk, s_slot, s_head;  // bytes
+};
+
+// Host plan of a launch.
+struct Mx4Plan {
+  int splits = 1;            // 16-row workgroups: splits of chunks_per_split chunks (0: dealt evenly)
+  int chunks_per_split = 0;
+  int pq_splits = 1;         // 64-row workgroups: key splits (chunks dealt evenly)
+  bool rows64 = false;       // requests of kPrefillRows rows or more in 64-row workgroups
+  int tok_cap = 0;           // AttnArgs::tok_cap
+};
+
+typedef const __attribute__((address_space(4))) int32_t* ConstI32;
+
+// Scale words of a row: D / 32 bytes.
+template <int D> struct Scales {
+  static constexpr int N = (D / 32 + 3) / 4;
+  uint32_t w[N];
+};
+template <int D> __device__ __forceinline__ Scales<D> load_scales(const uint8_t* p) {
+  Scales<D> s;
+  if constexpr (D == 64) {
+    s.w[0] = *reinterpret_cast<const uint16_t*>(p);
+  } else if constexpr (D == 128) {
+    s.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+    s.w[0] = v[0];
+    s.w[1] = v[1];
+  }
+  return s;
+}
+// A lane group's units of a row: D / 8 bytes.
+template <int D> struct Units {
+  uint32_t w[D / 32];
+};
+template <int D> __device__ __forceinline__ Units<D> load_units(const uint8_t* p) {
+  Units<D> u;
+  if constexpr (D == 64) {
+    const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+    u.w[0] = v[0];
+    u.w[1] = v[1];
+  } else {
+#pragma unroll
+    for (int j = 0; j < D / 32; j += 4) {
+      const u32x4 v = reinterpret_cast<const u32x4*>(p)[j / 4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u.w[j + i] = v[i];
+    }
+  }
+  return u;
+}
+
+// LDS rows of 16-byte chunks, chunk c of row r at slot c ^ swz(r).
+template <int D> struct Lds {
+  static constexpr int ROWB = D * 2, TILEB = TILE * ROWB;
+  static __device__ __forceinline__ int vswz(int r) { return DmaGeom<D>::swz(r); }
+  static __device__ __forceinline__ int kswz(int r) { return PDmaGeom<D>::kswz(r); }
+};
+
+__device__ __forceinline__ u32x4 lds_load16(const unsigned char* p) { return *reinterpret_cast<const u32x4*>(p); }
+__device__ __forceinline__ void lds_store16(unsigned char* p, u32x4 v) { *reinterpret_cast<u32x4*>(p) = v; }
+__device__ __forceinline__ u32x2 lds_load_tr8(const unsigned char* p) {
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(
+      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(p)));
+}
+
+// A workgroup barrier that orders LDS but waits for no global load in flight.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+// Orders a wave's LDS writes before its other lanes' reads (the LDS serves a
+// wave's accesses in order).
+__device__ __forceinline__ void lds_wave_order() {
+  __builtin_amdgcn_wave_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The paged cache as the kernels address it: 16-key granules, each within one
+// page (pages hold 16, 32, ... keys), their block-table entries by scalar
+// loads. Keys past the sequence read its last one (their scores are masked),
+// table and block indices are clamped into range, so inconsistent metadata
+// cannot address outside the cache.
+struct Pager {
+  ConstI32 row;
+  int last_key, last_block, max_blocks, ps_shift, page_mask;
+  __device__ __forceinline__ int granule(int g) const { return min(g, last_key >> 4); }
+  // the table entry of (clamped) granule g
+  __device__ __forceinline__ int entry(int g) const {
+    return row[uint32_t(min((16 * g) >> ps_shift, max_blocks - 1))];
+  }
+  __device__ __forceinline__ uint32_t block(int e) const { return uint32_t(e < 0 ? 0 : min(e, last_block)); }
+  // byte offset of granule g's first row
+  __device__ __forceinline__ uint64_t offset(int g, int e, uint32_t blk, uint32_t slot, uint32_t head_off) const {
+    return uint64_t(block(e)) * blk + uint64_t(uint32_t((16 * g) & page_mask)) * slot + head_off;
+  }
+};
+
+template <class A> __device__ __forceinline__ Pager make_pager(const A& a, int r, int seq_len) {
+  Pager p;
+  p.row = (ConstI32)(a.bt + int64_t(r) * a.sbt);
+  p.last_key = max(seq_len - 1, 0);
+  p.last_block = int(a.num_blocks - 1 < 0x7fffffff ? a.num_blocks - 1 : 0x7fffffff);
+  p.max_blocks = a.max_blocks;
+  p.ps_shift = a.ps_shift;
+  p.page_mask = a.page_size - 1;
+  return p;
+}
+
+// ---------------------------------------------------------------------------
+// 16 query rows. Wave w takes tiles w and w + 4 of a chunk: K fragments go
+// from global memory straight into the score MFMAs, V rows through a 32-key
+// LDS stage of the wave's own (unpacked, then read transposed). Per chunk two
+// barriers: the row maxima, and the waves' integer partial sums, which are
+// added in any order to the same bits (attn_impl.h's waves split them by d
+// instead). Loads run a phase ahead: a chunk's V goes out before its scores,
+// the next chunk's K before the weights.
+template <int DT, int BITS, int D, bool SPLIT>
+__global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn_mx4_rows16_kernel(Mx4Args m) {
+  const AttnArgs& a = m.a;
+  using TR = Traits<DT>;
+  using T = typename TR::T;
+  using AccT = typename AccOf<BITS>::T;
+  using L = Lds<D>;
+  constexpr int QS = D / 32, DBLK = D / 16, NT = CT / 4;
+  constexpr int VPT = D / 16;                      // accumulators per thread: 16 rows x D over 256 threads
+  constexpr int STAGEB = 32 * L::ROWB;             // the wave's V stage
+  constexpr int PARTB = QROWS * D * int(sizeof(AccT));  // the wave's partial sums, in the stage's place
+  constexpr int WAVEB = STAGEB > PARTB ? STAGEB : PARTB;
+  __shared__ __align__(16) unsigned char stage_all[4 * WAVEB];
+  __shared__ float red_m[2][4][QROWS];  // (by the chunk's parity: no third barrier)
+  __shared__ AccT red_d[4][QROWS];
+
+  const int tid = threadIdx.x, lane = tid & 63, kg = lane >> 4, i16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  unsigned char* stage = stage_all + wave * WAVEB;
+  const int r = blockIdx.x / a.num_kv_heads, g = blockIdx.x % a.num_kv_heads;
+  const int split = blockIdx.z;
+  const int q_start = ((ConstI32)a.qsl)[r];
+  const int q_len = ((ConstI32)a.qsl)[r + 1] - q_start;
+  const int seq_len = ((ConstI32)a.seq_lens)[r];
+  const int ctx = seq_len - q_len;
+  const int rows_total = q_len * a.group;
+  const int row0 = blockIdx.y * QROWS;
+  if (row0 >= rows_total) return;                          // uniform
+  if (a.pq_rows > 0 && rows_total >= a.pq_rows) return;  // attn_mx4_rows64_kernel's request
+  auto ws_row = [&](int64_t token) { return a.tok_cap > 0 ? int64_t(r) * a.tok_cap + (token - q_start) : token; };
+
+  const int i_min = row0 / a.group;
+  const int i_max = min(rows_total - 1, row0 + QROWS - 1) / a.group;
+  const int hi = a.causal ? min(seq_len, ctx + i_max + 1) : seq_len;
+  const int lo = a.window > 0 ? max(0, ctx + i_min - a.window + 1) : 0;
+  const int t_lo = lo / TILE;
+  const int t_hi = hi > lo ? (hi + TILE - 1) / TILE : t_lo;
+  const int c_first = t_lo / CT;
+  int c_end = t_hi > t_lo ? (t_hi + CT - 1) / CT : c_first;
+  if constexpr (SPLIT) c_end = min(c_end, a.chunk_slots);
+  const int nch = max(0, c_end - c_first);
+  const int per = !SPLIT ? nch : a.chunks_per_split > 0 ? a.chunks_per_split : (nch + a.num_splits - 1) / a.num_splits;
+  const int c_lo = c_first + min(nch, (SPLIT ? split : 0) * per);
+  const int c_hi = min(c_first + nch, c_lo + per);
+
+  // the thread's part of the sums: row tid / 16, elements VPT (tid % 16) ..
+  const RowInfo mine = row_info(a, g, q_start, q_len, ctx, seq_len, row0 + (tid >> 4));
+  const int my_d = VPT * (tid & 15);
+  if (SPLIT && split == 0 && (tid & 15) == 0 && mine.valid) {
+    int* cr = a.crange + 2 * (ws_row(mine.token) * a.num_heads + mine.head);
+    cr[0] = c_first;
+    cr[1] = c_first + nch;
+  }
+  if (SPLIT && c_lo >= c_hi) return;  // uniform
+
+  const Pager pager = make_pager(a, r, seq_len);
+  const uint32_t ch = uint32_t(g) * m.c_head, sh = uint32_t(g) * m.s_head;
+
+  // The lane's query row (a column of the score MFMAs).
+  const RowInfo me = row_info(a, g, q_start, q_len, ctx, seq_len, row0 + i16);
+  u32x4 qf[QS];
+  {
+    const T* qbase = static_cast<const T*>(a.q) + me.token * a.sq_t + int64_t(me.head) * a.sq_h;
+#pragma unroll
+    for (int j = 0; j < QS; ++j)
+      qf[j] = me.valid ? *reinterpret_cast<const u32x4*>(qbase + 32 * j + 8 * kg) : u32x4{0u, 0u, 0u, 0u};
+  }
+  const int ks = me.valid ? me.kstart : 0x7fffffff;
+  const int ke = me.valid ? me.kend : 0;
+  const int qp = me.qpos;
+  const float slope = a.alibi ? a.alibi[me.head] : 0.0f;
+
+  auto live_lo = [&](int c) { return max(c * CT, t_lo); };
+  auto live_hi = [&](int c) { return min(c * CT + CT, t_hi); };
+  // the wave's tile u (0, 1) of chunk c, moved onto a live one (whose loads are
+  // in flight anyway) where it is none
+  auto tile_of = [&](int c, int u) { return min(max(c * CT + wave + 4 * u, live_lo(c)), live_hi(c) - 1); };
+
+  int ent[NT][4];  // table entries of the granules of the wave's tiles
+  auto load_entries = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) ent[u][q] = pager.entry(pager.granule(4 * tile_of(c, u) + q));
+  };
+
+  // K: MFMA row i16 of (s, h) is the tile's key 32 s + pi(i16, h), in granule
+  // 2 s + i16 / 8.
+  Units<D> kb[NT][4];
+  Scales<D> kbs[NT][4];
+  auto load_k = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int t = tile_of(c, u);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int g0 = pager.granule(4 * t + 2 * s), g1 = pager.granule(4 * t + 2 * s + 1);
+        const uint64_t c0 = pager.offset(g0, ent[u][2 * s], m.c_blk, m.c_slot, ch);
+        const uint64_t c1 = pager.offset(g1, ent[u][2 * s + 1], m.c_blk, m.c_slot, ch);
+        const uint64_t s0 = pager.offset(g0, ent[u][2 * s], m.s_blk, m.s_slot, sh);
+        const uint64_t s1 = pager.offset(g1, ent[u][2 * s + 1], m.s_blk, m.s_slot, sh);
+        const bool up = i16 >= 8;
+        const uint8_t* cp = m.kc + (up ? c1 : c0) + kg * (D / 8);
+        const uint8_t* sp = m.ks + (up ? s1 : s0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int key = t * TILE + 32 * s + 8 * (i16 >> 2) + 4 * h + (i16 & 3);
+          const uint32_t in = uint32_t(min(key, pager.last_key) - 16 * (up ? g1 : g0));
+          kb[u][2 * s + h] = load_units<D>(cp + in * m.c_slot);
+          kbs[u][2 * s + h] = load_scales<D>(sp + in * m.s_slot);
+        }
+      }
+    }
+  };
+  // V: lane l of load q has row 16 q + l / 4 of the tile, units l % 4.
+  Units<D> vb[NT][4];
+  Scales<D> vbs[NT][4];
+  auto load_v = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int t = tile_of(c, u);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int gq = pager.granule(4 * t + q);
+        const uint8_t* cp = m.vc + pager.offset(gq, ent[u][q], m.c_blk, m.c_slot, ch);
+        const uint8_t* sp = m.vs + pager.offset(gq, ent[u][q], m.s_blk, m.s_slot, sh);
+        const int key = t * TILE + 16 * q + (lane >> 2);
+        const uint32_t in = uint32_t(min(key, pager.last_key) - 16 * gq);
+        vb[u][q] = load_units<D>(cp + (in * m.c_slot + (lane & 3) * (D / 8)));
+        vbs[u][q] = load_scales<D>(sp + in * m.s_slot);
+      }
+    }
+  };
+
+  // LDS addresses of the V stage: the row and chunk slots the lane writes, and
+  // its transposing reads (keys 8 kg + j / 4 + 4 h, columns 4 (j % 4) of d block
+  // 0; d block db is at ^ (db << 5)).
+  const int wr = lane >> 2;
+  unsigned vrd[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int rr = 8 * kg + (i16 >> 2) + 4 * h;
+    vrd[h] = rr * L::ROWB + ((((i16 & 3) >> 1) ^ L::vswz(rr)) << 4) + (i16 & 1) * 8;
+  }
+
+  float M = -__builtin_inff();  // the thread's row, folded
+  AccT Dn = 0, W[VPT];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) W[v] = 0;
+
+  if (c_lo < c_hi) {
+    load_entries(c_lo);
+    load_k(c_lo);
+    for (int c = c_lo;; ++c) {
+      const int ta = live_lo(c), te = live_hi(c);
+      load_v(c);
+      if (c + 1 < c_hi) load_entries(c + 1);
+
+      // scores of the wave's tiles, for the lane's row and keys 32 s + 8 kg + 4 h + e
+      float sc[NT][4][4];
+      float mx = -__builtin_inff();
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const int t = c * CT + wave + 4 * u;
+        const bool live = t >= ta && t < te;  // uniform
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < QS; ++j)
+            acc = TR::mma(mx4::unpack8<DT>(kb[u][q].w[j], mx4::scale_of<DT>(kbs[u][q].w[j / 4], j % 4)), qf[j], acc);
+          const int key0 = t * TILE + 32 * (q >> 1) + 8 * kg + 4 * (q & 1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = __fmul_rn(acc[e], a.scale_log2);
+            if (a.softcap_log2 > 0.0f) x = softcapped(x, a.softcap_log2);
+            if (a.alibi) x = x + slope * static_cast<float>(key0 + e - qp);
+            sc[u][q][e] = (live && key0 + e >= ks && key0 + e < ke) ? x : -__builtin_inff();
+            mx = fmaxf(mx, sc[u][q][e]);
+          }
+        }
+      }
+      if (c + 1 < c_hi) load_k(c + 1);
+
+      // the chunk's row maxima: the row's four lanes, then the waves
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      float(&rm)[4][QROWS] = red_m[c & 1];
+      if (kg == 0) rm[wave][i16] = mx;
+      lds_barrier();
+      mx = fmaxf(fmaxf(rm[0][i16], rm[1][i16]), fmaxf(rm[2][i16], rm[3][i16]));
+      const float mrow = mx != -__builtin_inff() ? mx : 0.0f;  // no key: pin to 0
+
+      // weights and weighted V of the wave's tiles
+      AccT den = 0;
+      AccT wv[DBLK][4];
+#pragma unroll
+      for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wv[b][e] = 0;
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const int t = c * CT + wave + 4 * u;
+        if (t >= ta && t < te) {  // uniform
+          f32x4 acc[DBLK];
+#pragma unroll
+          for (int b = 0; b < DBLK; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            u32x4 pb;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t p16[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float w = __builtin_amdgcn_exp2f(sc[u][2 * s + h][e] - mrow);
+                den = wadd<BITS>(den, quant<BITS>(__fmul_rn(w, a.fxp_scale)));
+                p16[e] = Io<DT>::store(w);
+              }
+              pb[2 * h] = p16[0] | (p16[1] << 16);
+              pb[2 * h + 1] = p16[2] | (p16[3] << 16);
+            }
+            lds_wave_order();
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int rr = 16 * q + wr;
+              unsigned char* row = stage + rr * L::ROWB;
+#pragma unroll
+              for (int j = 0; j < QS; ++j)
+                lds_store16(row + (((4 * j + (lane & 3)) ^ L::vswz(rr)) << 4),
+                            mx4::unpack8<DT>(vb[u][2 * s + q].w[j],
+                                             mx4::scale_of<DT>(vbs[u][2 * s + q].w[j / 4], j % 4)));
+            }
+            lds_wave_order();
+#pragma unroll
+            for (int b = 0; b < DBLK; ++b) {
+              const u32x2 lo2 = lds_load_tr8(stage + (vrd[0] ^ (b << 5)));
+              const u32x2 hi2 = lds_load_tr8(stage + (vrd[1] ^ (b << 5)));
+              acc[b] = TR::mma(u32x4{lo2[0], lo2[1], hi2[0], hi2[1]}, pb, acc[b]);
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) wv[b][e] = wadd<BITS>(wv[b][e], quant<BITS>(__fmul_rn(acc[b][e], a.fxp_scale)));
+        }
+      }
+
+      // the waves' partial sums to LDS: lane (kg, row) holds d = 16 b + 4 kg + e
+      den = wadd<BITS>(den, __shfl_xor(den, 16, 64));
+      den = wadd<BITS>(den, __shfl_xor(den, 32, 64));
+      if (kg == 0) red_d[wave][i16] = den;
+      lds_wave_order();
+      {
+        typedef AccT acc4 __attribute__((ext_vector_type(4)));
+        acc4* p = reinterpret_cast<acc4*>(stage) + i16 * (D / 4);
+#pragma unroll
+        for (int b = 0; b < DBLK; ++b) p[4 * b + kg] = acc4{wv[b][0], wv[b][1], wv[b][2], wv[b][3]};
+      }
+      lds_barrier();
+      {
+        const int row = tid >> 4;
+        AccT cd = wadd<BITS>(wadd<BITS>(red_d[0][row], red_d[1][row]), wadd<BITS>(red_d[2][row], red_d[3][row]));
+        const float cm = fmaxf(fmaxf(rm[0][row], rm[1][row]), fmaxf(rm[2][row], rm[3][row]));
+        AccT cw[VPT];
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+          cw[v] = 0;
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            cw[v] = wadd<BITS>(cw[v], reinterpret_cast<const AccT*>(stage_all + w * WAVEB)[row * D + my_d + v]);
+        }
+        if constexpr (SPLIT) {
+          if (mine.valid) {
+            const int64_t slot = (ws_row(mine.token) * a.num_heads + mine.head) * a.chunk_slots + c;
+            if ((tid & 15) == 0) {
+              a.pmax[slot] = cm;
+              static_cast<AccT*>(a.den_ws)[slot] = cd;
+            }
+            AccT* wp = static_cast<AccT*>(a.wv_ws) + slot * D + my_d;
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) wp[v] = cw[v];
+          }
+        } else if (cm != -__builtin_inff()) {
+          float Mn, fa, fb;
+          merge_factors(M, cm, Mn, fa, fb);
+          Dn = wadd<BITS>(rescale<BITS>(Dn, fa), rescale<BITS>(cd, fb));
+#pragma unroll
+          for (int v = 0; v < VPT; ++v) W[v] = wadd<BITS>(rescale<BITS>(W[v], fa), rescale<BITS>(cw[v], fb));
+          M = Mn;
+        }
+      }
+      // (the next chunk's first barrier stands between these reads and the
+      // next writes of the stages and of red_d)
+      if (c + 1 >= c_hi) break;
+    }
+  }
+
+  if constexpr (!SPLIT) {
+    if (mine.valid) {
+      const float den_f = fmaxf(acc_f32<BITS>(Dn, a.fxp_inv), 1.0e-6f);
+      T* o = static_cast<T*>(a.o) + mine.token * a.so_t + int64_t(mine.head) * a.so_h + my_d;
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) o[v] = Io<DT>::store(div_rn(acc_f32<BITS>(W[v], a.fxp_inv), den_f));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// 64 query rows, 16 a wave. A chunk's K tiles are read twice, for the row
+// maxima (two tiles a step) and, with the V tiles, for the weights, as in
+// attn_impl.h's prefill kernels. A step has two tiles in LDS (K K or K V) and
+// the next step's two in registers, packed: they are unpacked into the other
+// two LDS tiles after the step's barrier, and the loads of the step after that
+// go out behind them.
+//
+// SPLIT: the chunks of a row tile are dealt evenly to pq_splits workgroups; the
+// first folds its chunks and leaves the folded state as one record, the others
+// a record per chunk.
+template <int DT, int BITS, int D, bool SPLIT>
+__global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void attn_mx4_rows64_kernel(Mx4Args m) {
+  const AttnArgs& a = m.a;
+  using TR = Traits<DT>;
+  using T = typename TR::T;
+  using AccT = typename AccOf<BITS>::T;
+  using L = Lds<D>;
+  constexpr int QS = D / 32, DBLK = D / 16;
+  extern __shared__ __align__(16) unsigned char lds[];  // [2][2] tiles
+
+  const int tid = threadIdx.x, lane = tid & 63, kg = lane >> 4, i16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = blockIdx.x % a.num_kv_heads;
+  int r = blockIdx.x / a.num_kv_heads, rtile = int(gridDim.y) - 1 - int(blockIdx.y);  // the longest row tiles first
+  if (a.pq_blocks > 0) {
+    r = __builtin_amdgcn_readfirstlane(flat_block(a, a.pq_blocks - 1 - r, rtile));
+    rtile = __builtin_amdgcn_readfirstlane(rtile);
+    if (r < 0 || rtile < 0) return;  // uniform
+  }
+  const int q_start = ((ConstI32)a.qsl)[r];
+  const int q_len = ((ConstI32)a.qsl)[r + 1] - q_start;
+  const int seq_len = ((ConstI32)a.seq_lens)[r];
+  const int ctx = seq_len - q_len;
+  const int rows_total = q_len * a.group;
+  const int row0 = rtile * PQROWS;
+  if (row0 >= rows_total || rows_total < a.pq_rows) return;  // uniform
+  const int wrow0 = row0 + 16 * wave;
+
+  const int i_min = row0 / a.group;
+  const int i_max = min(rows_total - 1, row0 + PQROWS - 1) / a.group;
+  const int hi = a.causal ? min(seq_len, ctx + i_max + 1) : seq_len;
+  const int lo = a.window > 0 ? max(0, ctx + i_min - a.window + 1) : 0;
+  const int t_lo = lo / TILE;
+  const int t_hi = hi > lo ? (hi + TILE - 1) / TILE : t_lo;
+  const int c_first = t_lo / CT;
+  int c_end = t_hi > t_lo ? (t_hi + CT - 1) / CT : c_first;
+  if constexpr (SPLIT) c_end = min(c_end, a.chunk_slots);
+  const int nch = max(0, c_end - c_first);
+  const int split = SPLIT ? blockIdx.z : 0;
+  const int per = SPLIT ? (nch + a.pq_splits - 1) / a.pq_splits : nch;
+  const int c_lo = c_first + min(nch, split * per);
+  const int c_hi = min(c_first + nch, c_lo + per);
+
+  const Pager pager = make_pager(a, r, seq_len);
+  const uint32_t ch = uint32_t(g) * m.c_head, sh = uint32_t(g) * m.s_head;
+
+  // The lane's query row.
+  const RowInfo me = row_info(a, g, q_start, q_len, ctx, seq_len, wrow0 + i16);
+  u32x4 qf[QS];
+  {
+    const T* qbase = static_cast<const T*>(a.q) + me.token * a.sq_t + int64_t(me.head) * a.sq_h;
+#pragma unroll
+    for (int j = 0; j < QS; ++j)
+      qf[j] = me.valid ? *reinterpret_cast<const u32x4*>(qbase + 32 * j + 8 * kg) : u32x4{0u, 0u, 0u, 0u};
+  }
+  const int ks = me.valid ? me.kstart : 0x7fffffff;
+  const int ke = me.valid ? me.kend : 0;
+  const int qp = me.qpos;
+  const float slope = a.alibi ? a.alibi[me.head] : 0.0f;
+
+  // Staging: the wave moves the tile's granule `wave`, lane l row l / 4, units
+  // l % 4.
+  struct Staged {
+    Units<D> u;
+    Scales<D> s;
+  };
+  const int srow = 16 * wave + (lane >> 2);
+  auto fetch = [&](bool isv, int t) __attribute__((always_inline)) {
+    const int gq = pager.granule(4 * t + wave);
+    const int e = pager.entry(gq);
+    const uint8_t* cp = (isv ? m.vc : m.kc) + pager.offset(gq, e, m.c_blk, m.c_slot, ch);
+    const uint8_t* sp = (isv ? m.vs : m.ks) + pager.offset(gq, e, m.s_blk, m.s_slot, sh);
+    const uint32_t in = uint32_t(min(t * TILE + srow, pager.last_key) - 16 * gq);
+    Staged x;
+    x.u = load_units<D>(cp + (in * m.c_slot + (lane & 3) * (D / 8)));
+    x.s = load_scales<D>(sp + in * m.s_slot);
+    return x;
+  };
+  auto put = [&](const Staged& x, unsigned char* tile, bool isv) __attribute__((always_inline)) {
+    unsigned char* row = tile + srow * L::ROWB;
+    const int sw = isv ? L::vswz(srow) : L::kswz(srow);
+#pragma unroll
+    for (int j = 0; j < QS; ++j)
+      lds_store16(row + (((4 * j + (lane & 3)) ^ sw) << 4),
+                  mx4::unpack8<DT>(x.u.w[j], mx4::scale_of<DT>(x.s.w[j / 4], j % 4)));
+  };
+
+  // LDS offsets of the score MFMAs' K rows pi(i16) (step s: + 32 rows, which
+  // the swizzle ignores) and of the transposing V reads, as in attn_impl.h.
+  unsigned koff[2][QS];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int j = 0; j < QS; ++j) {
+      const int rr = 8 * (i16 >> 2) + 4 * h + (i16 & 3);
+      koff[h][j] = rr * L::ROWB + (((4 * j + kg) ^ L::kswz(rr)) << 4);
+    }
+  unsigned vrd[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int rr = 8 * kg + (i16 >> 2) + 4 * h;
+    vrd[h] = rr * L::ROWB + ((((i16 & 3) >> 1) ^ L::vswz(rr)) << 4) + (i16 & 1) * 8;
+  }
+
+  float Mr = -__builtin_inff();
+  AccT Dr = 0;
+  AccT Wr[DBLK][4];
+#pragma unroll
+  for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) Wr[b][e] = 0;
+
+  auto store_record = [&](int c, float mc, AccT den, const AccT (&w)[DBLK][4]) __attribute__((always_inline)) {
+    if (!me.valid) return;
+    const int64_t slot = (me.token * a.num_heads + me.head) * a.chunk_slots + c;
+    if (kg == 0) {
+      a.pmax[slot] = mc;
+      static_cast<AccT*>(a.den_ws)[slot] = den;
+    }
+    typedef AccT acc4 __attribute__((ext_vector_type(4)));
+    acc4* wp = reinterpret_cast<acc4*>(static_cast<AccT*>(a.wv_ws) + slot * D + 4 * kg);
+#pragma unroll
+    for (int b = 0; b < DBLK; ++b) wp[4 * b] = acc4{w[b][0], w[b][1], w[b][2], w[b][3]};
+  };
+
+  auto live_lo = [&](int c) { return max(c * CT, t_lo); };
+  auto live_hi = [&](int c) { return min(c * CT + CT, t_hi); };
+  // The steps of chunk c: phase 0 takes K tiles ta + 2 k, ta + 2 k + 1 (the last
+  // one twice where they are odd), phase 1 K and V of tile ta + k.
+  struct Step {
+    int c, phase, k;
+  };
+  auto next = [&](Step s) {
+    const int n = live_hi(s.c) - live_lo(s.c);
+    ++s.k;
+    if (s.phase == 0 && 2 * s.k >= n) {
+      s.phase = 1;
+      s.k = 0;
+    } else if (s.phase == 1 && s.k >= n) {
+      if (s.c + 1 < c_hi) {
+        ++s.c;
+        s.phase = 0;
+        s.k = 0;
+      } else {
+        s.k = n - 1;  // past the end: the last step again
+      }
+    }
+    return s;
+  };
+  Staged r0, r1;
+  auto fetch_step = [&](const Step& s) __attribute__((always_inline)) {
+    const int ta = live_lo(s.c), te = live_hi(s.c);
+    const bool kv = s.phase == 1;
+    r0 = fetch(false, ta + (kv ? s.k : 2 * s.k));
+    r1 = fetch(kv, kv ? ta + s.k : min(ta + 2 * s.k + 1, te - 1));
+  };
+  int buf = 0;
+  auto tile_at = [&](int b, int j) { return lds + (2 * b + j) * L::TILEB; };
+
+  auto scores_of = [&](const unsigned char* tile, auto&& fn) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < QS; ++j)
+        acc = TR::mma(lds_load16(tile + (q >> 1) * 32 * L::ROWB + koff[q & 1][j]), qf[j], acc);
+      fn(q, acc);
+    }
+  };
+  auto masked = [&](const f32x4& acc, int t, int q, float (&sc)[4]) __attribute__((always_inline)) {
+    const int key0 = t * TILE + 32 * (q >> 1) + 8 * kg + 4 * (q & 1);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x = __fmul_rn(acc[e], a.scale_log2);
+      if (a.softcap_log2 > 0.0f) x = softcapped(x, a.softcap_log2);
+      if (a.alibi) x = x + slope * static_cast<float>(key0 + e - qp);
+      sc[e] = (key0 + e >= ks && key0 + e < ke) ? x : -__builtin_inff();
+    }
+  };
+
+  if (c_lo < c_hi) {
+    Step cur{c_lo, 0, 0}, ahead = next(cur);
+    fetch_step(cur);
+    put(r0, tile_at(0, 0), false);
+    put(r1, tile_at(0, 1), false);
+    fetch_step(ahead);
+    // One step: publish its tiles, unpack the next step's, load the one after.
+    auto step_begin = [&]() __attribute__((always_inline)) {
+      lds_barrier();
+      put(r0, tile_at(buf ^ 1, 0), false);
+      put(r1, tile_at(buf ^ 1, 1), ahead.phase == 1);
+      cur = ahead;
+      ahead = next(ahead);
+      fetch_step(ahead);
+    };
+    for (int c = c_lo; c < c_hi; ++c) {
+      const int ta = live_lo(c), te = live_hi(c);
+      float mx = -__builtin_inff();
+      for (int t = ta; t < te; t += 2) {
+        step_begin();
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (t + j < te)
+            scores_of(tile_at(buf, j), [&](int q, const f32x4& acc) __attribute__((always_inline)) {
+              float sc[4];
+              masked(acc, t + j, q, sc);
+              mx = fmaxf(fmaxf(mx, fmaxf(sc[0], sc[1])), fmaxf(sc[2], sc[3]));
+            });
+        }
+        buf ^= 1;
+      }
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mrow = mx != -__builtin_inff() ? mx : 0.0f;  // no key: pin to 0
+      AccT den = 0;
+      AccT wv[DBLK][4];
+#pragma unroll
+      for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wv[b][e] = 0;
+      for (int t = ta; t < te; ++t) {
+        step_begin();
+        u32x4 pb[2];
+        scores_of(tile_at(buf, 0), [&](int q, const f32x4& acc) __attribute__((always_inline)) {
+          float sc[4];
+          masked(acc, t, q, sc);
+          uint32_t p16[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float w = __builtin_amdgcn_exp2f(sc[e] - mrow);
+            den = wadd<BITS>(den, quant<BITS>(__fmul_rn(w, a.fxp_scale)));
+            p16[e] = Io<DT>::store(w);
+          }
+          pb[q >> 1][2 * (q & 1)] = p16[0] | (p16[1] << 16);
+          pb[q >> 1][2 * (q & 1) + 1] = p16[2] | (p16[3] << 16);
+        });
+        const unsigned char* vt = tile_at(buf, 1);
+#pragma unroll
+        for (int b = 0; b < DBLK; ++b) {
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const u32x2 lo2 = lds_load_tr8(vt + s * 32 * L::ROWB + (vrd[0] ^ (b << 5)));
+            const u32x2 hi2 = lds_load_tr8(vt + s * 32 * L::ROWB + (vrd[1] ^ (b << 5)));
+            acc = TR::mma(u32x4{lo2[0], lo2[1], hi2[0], hi2[1]}, pb[s], acc);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) wv[b][e] = wadd<BITS>(wv[b][e], quant<BITS>(__fmul_rn(acc[e], a.fxp_scale)));
+        }
+        buf ^= 1;
+      }
+      den = wadd<BITS>(den, __shfl_xor(den, 16, 64));
+      den = wadd<BITS>(den, __shfl_xor(den, 32, 64));
+      if (SPLIT && split > 0) {  // uniform
+        store_record(c, mx, den, wv);
+      } else if (mx != -__builtin_inff()) {
+        float Mn, fa, fb;
+        merge_factors(Mr, mx, Mn, fa, fb);
+        Dr = wadd<BITS>(rescale<BITS>(Dr, fa), rescale<BITS>(den, fb));
+#pragma unroll
+        for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) Wr[b][e] = wadd<BITS>(rescale<BITS>(Wr[b][e], fa), rescale<BITS>(wv[b][e], fb));
+        Mr = Mn;
+      }
+    }
+  }
+
+  if constexpr (SPLIT) {
+    if (split == 0) {
+      if (c_lo < c_hi) store_record(c_hi - 1, Mr, Dr, Wr);
+      if (me.valid && kg == 0) {
+        int* cr = a.crange + 2 * (me.token * a.num_heads + me.head);
+        cr[0] = c_lo < c_hi ? c_hi - 1 : c_first;
+        cr[1] = c_end;
+      }
+    }
+  } else if (me.valid) {
+    const float den_f = fmaxf(acc_f32<BITS>(Dr, a.fxp_inv), 1.0e-6f);
+    T* orow = static_cast<T*>(a.o) + me.token * a.so_t + int64_t(me.head) * a.so_h;
+#pragma unroll
+    for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        orow[b * 16 + 4 * kg + e] = Io<DT>::store(div_rn(acc_f32<BITS>(Wr[b][e], a.fxp_inv), den_f));
+  }
+}
+
+// Folds the records of each (token, head) in ascending chunk order and divides:
+// a thread takes two consecutive d of a row.
+template <int DT, int BITS, int D>
+__global__ __launch_bounds__(256) void attn_mx4_combine_kernel(AttnArgs a) {
+  using T = typename Traits<DT>::T;
+  using AccT = typename AccOf<BITS>::T;
+  constexpr int V = 2, PER = D / V;
+  typedef AccT accv __attribute__((ext_vector_type(V)));
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t th = idx / PER;
+  const int d = int(idx % PER) * V;
+  const uint32_t wrow = th / uint32_t(a.num_heads);
+  const int head = int(th - wrow * uint32_t(a.num_heads));
+  int64_t token = wrow;
+  if (a.tok_cap > 0) {
+    const uint32_t r = wrow / uint32_t(a.tok_cap);
+    if (r >= uint32_t(a.num_requests)) return;
+    const int i = int(wrow - r * uint32_t(a.tok_cap)), q0 = a.qsl[r], q_len = a.qsl[r + 1] - q0;
+    if (i >= q_len || (a.pq_rows > 0 && q_len * a.group >= a.pq_rows)) return;
+    token = q0 + i;
+    if (token < 0 || token >= a.num_tokens) return;
+  } else {
+    // tokens outside query_start_loc's range belong to no request and are left
+    // as they are
+    const int64_t used = min<int64_t>(a.num_tokens, a.qsl[a.num_requests]);
+    if (token < a.qsl[0] || token >= used) return;
+  }
+  const int c0 = max(0, a.crange[2 * int64_t(th)]), c1 = min(a.chunk_slots, a.crange[2 * int64_t(th) + 1]);
+  const AccT* den_p = static_cast<const AccT*>(a.den_ws) + int64_t(th) * a.chunk_slots;
+  const AccT* wv_p = static_cast<const AccT*>(a.wv_ws) + int64_t(th) * a.chunk_slots * D + d;
+  const float* pm_p = a.pmax + int64_t(th) * a.chunk_slots;
+  float M = -__builtin_inff();
+  AccT Dn = 0, W[V] = {0, 0};
+  constexpr int NB = 8;
+  for (int cb = c0; cb < c1; cb += NB) {
+    float mc[NB];
+    AccT dc[NB];
+    accv wc[NB];
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const int c = min(cb + k, c1 - 1);
+      mc[k] = pm_p[c];
+      dc[k] = den_p[c];
+      wc[k] = *reinterpret_cast<const accv*>(wv_p + int64_t(c) * D);
+    }
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      if (cb + k >= c1 || mc[k] == -__builtin_inff()) continue;
+      float Mn, fa, fb;
+      merge_factors(M, mc[k], Mn, fa, fb);
+      Dn = wadd<BITS>(rescale<BITS>(Dn, fa), rescale<BITS>(dc[k], fb));
+#pragma unroll
+      for (int v = 0; v < V; ++v) W[v] = wadd<BITS>(rescale<BITS>(W[v], fa), rescale<BITS>(wc[k][v], fb));
+      M = Mn;
+    }
+  }
+  const float den_f = fmaxf(acc_f32<BITS>(Dn, a.fxp_inv), 1.0e-6f);
+  T* o = static_cast<T*>(a.o) + token * a.so_t + int64_t(head) * a.so_h + d;
+#pragma unroll
+  for (int v = 0; v < V; ++v) o[v] = Io<DT>::store(div_rn(acc_f32<BITS>(W[v], a.fxp_inv), den_f));
+}
+
+// ---------------------------------------------------------------------------
+// Launches.
+
+template <int DT, int BITS, int D, bool SPLIT> int launch_rows64(const Mx4Args& m, dim3 grid, hipStream_t st) {
+  auto kern = attn_mx4_rows64_kernel<DT, BITS, D, SPLIT>;
+  constexpr int lds = 4 * Lds<D>::TILEB;
+  static bool attr_done = false;  // benign race: the attribute is idempotent
+  if (!attr_done) {
+    const hipError_t e =
+        hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return int(e);
+    attr_done = true;
+  }
+  kern<<<grid, kPThreads, lds, st>>>(m);
+  return 0;
+}
+
+template <int DT, int BITS, int D>
+int launch_mx4(Mx4Args m, const Mx4Plan& p, int num_requests, int max_query_len, int64_t num_tokens, hipStream_t st) {
+  AttnArgs& a = m.a;
+  a.num_splits = p.splits;
+  a.chunks_per_split = p.chunks_per_split;
+  a.pq_splits = p.pq_splits;
+  a.tok_cap = p.tok_cap;
+  const int64_t max_rows = int64_t(max_query_len > 1 ? max_query_len : 1) * a.group;
+  const bool split = p.splits > 1 || p.pq_splits > 1;
+  int64_t qtiles = cdiv(max_rows, QROWS);
+  if (p.rows64) {
+    a.pq_rows = kPrefillRows;
+    qtiles = std::min<int64_t>(qtiles, kShortTiles);
+    const int64_t ptiles = cdiv(max_rows, PQROWS);
+    // a flat grid over the tokens where requests x the longest one's tiles
+    // would be mostly empty
+    const int64_t flat = num_tokens * a.group / PQROWS + num_requests;
+    dim3 grid(unsigned(num_requests * a.num_kv_heads), unsigned(ptiles), unsigned(p.pq_splits));
+    if (ptiles > 65535 || (num_requests * ptiles - flat) * a.num_kv_heads * p.pq_splits > kFlatEmpty) {
+      a.pq_blocks = int(flat);
+      grid = dim3(unsigned(flat * a.num_kv_heads), 1, unsigned(p.pq_splits));
+    }
+    const int e = p.pq_splits > 1 ? launch_rows64<DT, BITS, D, true>(m, grid, st)
+                                  : launch_rows64<DT, BITS, D, false>(m, grid, st);
+    if (e) return e;
+  }
+  const dim3 grid(unsigned(num_requests * a.num_kv_heads), unsigned(qtiles), unsigned(p.splits));
+  if (!split) {
+    attn_mx4_rows16_kernel<DT, BITS, D, false><<<grid, kThreads, 0, st>>>(m);
+    return launch_status();
+  }
+  attn_mx4_rows16_kernel<DT, BITS, D, true><<<grid, kThreads, 0, st>>>(m);
+  const int64_t ws_rows = a.tok_cap > 0 ? int64_t(num_requests) * a.tok_cap : num_tokens;
+  attn_mx4_combine_kernel<DT, BITS, D>
+      <<<dim3(unsigned(cdiv(ws_rows * a.num_heads * (D / 2), 256))), 256, 0, st>>>(a);
+  return launch_status();
+}
+
+template <int DT, int BITS>
+int dispatch_d(const Mx4Args& m, const Mx4Plan& p, int num_requests, int max_query_len, int64_t num_tokens, hipStream_t st) {
+  switch (m.a.head_dim) {
+    case 64: return launch_mx4<DT, BITS, 64>(m, p, num_requests, max_query_len, num_tokens, st);
+    case 128: return launch_mx4<DT, BITS, 128>(m, p, num_requests, max_query_len, num_tokens, st);
+    default: return launch_mx4<DT, BITS, 256>(m, p, num_requests, max_query_len, num_tokens, st);
+  }
+}
+
+int run_mx4_bf16(const Mx4Args& m, const Mx4Plan& p, int bits, int num_requests, int max_query_len, int64_t num_tokens,
+                 hipStream_t st);
+int run_mx4_f16(const Mx4Args& m, const Mx4Plan& p, int bits, int num_requests, int max_query_len, int64_t num_tokens,
+                hipStream_t st);
+
+}  // namespace m4
+}  // namespace attn
+}  // namespace fxpr

@@ -17,6 +17,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <optional>
@@ -337,6 +338,165 @@ void reshape_and_cache(const Tensor& key_in, const Tensor& value_in, Tensor& kv_
            "fxpr_reshape_and_cache");
 }
 
+// The cache in 4 bits (fxpr_vllm/_kernels/mx4.py).
+bool mx4_head_size(int64_t d) { return d == 64 || d == 128 || d == 256; }
+
+void check_mx4_cache(const char* what, const Tensor& codes, const Tensor& scales) {
+  TORCH_CHECK(codes.is_cuda() && scales.is_cuda(), what, ": tensors must be CUDA");
+  TORCH_CHECK_TYPE(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte, what,
+                   ": kv_codes and kv_scales must be uint8");
+  TORCH_CHECK_VALUE(codes.dim() == 5 && codes.size(1) == 2, what,
+                    ": kv_codes must be (num_blocks, 2, block_size, num_kv_heads, head_size / 2)");
+  TORCH_CHECK_VALUE(mx4_head_size(2 * codes.size(4)), what, ": head_size must be one of 64, 128, 256, got ",
+                    2 * codes.size(4));
+  TORCH_CHECK_VALUE(scales.dim() == 5 && scales.sizes().slice(0, 4) == codes.sizes().slice(0, 4) &&
+                        scales.size(4) * 16 == codes.size(4),
+                    what, ": kv_scales must be (num_blocks, 2, block_size, num_kv_heads, head_size / 32)");
+  TORCH_CHECK_VALUE(codes.stride(4) == 1 && scales.stride(4) == 1, what,
+                    ": kv_codes and kv_scales must be contiguous along a row");
+}
+
+template <class... Ts> void check_same_device(const char* what, const Tensor& first, const Ts&... others) {
+  TORCH_CHECK(((others.device() == first.device()) && ...), what, ": tensors must be on one device");
+}
+
+// [tokens, heads, head_size] with 16-byte aligned rows (a copy where they are not)
+Tensor aligned_rows(const Tensor& t) {
+  const int64_t n = t.element_size();
+  const bool ok = t.stride(2) == 1 && t.stride(0) * n % 16 == 0 && t.stride(1) * n % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+Tensor mx4_slots(const char* what, const Tensor& slot_mapping, int64_t least) {
+  TORCH_CHECK_TYPE(slot_mapping.scalar_type() == at::kInt || slot_mapping.scalar_type() == at::kLong, what,
+                   ": slot_mapping must be int32 or int64");
+  TORCH_CHECK_VALUE(slot_mapping.dim() == 1 && slot_mapping.size(0) >= least, what,
+                    ": slot_mapping must be 1-D with one slot per token");
+  return slot_mapping.to(at::kLong).contiguous();
+}
+
+void reshape_and_cache_mx4(const Tensor& key_in, const Tensor& value_in, Tensor& codes, Tensor& scales,
+                           const Tensor& slot_mapping) {
+  const char* what = "reshape_and_cache_mx4";
+  TORCH_CHECK(key_in.is_cuda() && value_in.is_cuda() && slot_mapping.is_cuda(), what, ": tensors must be CUDA");
+  check_mx4_cache(what, codes, scales);
+  const auto t = key_in.scalar_type();
+  TORCH_CHECK_TYPE(is_io(t), what, ": unsupported dtype ", t, "; expected float16, bfloat16 or float32");
+  TORCH_CHECK_TYPE(value_in.scalar_type() == t, what, ": key and value must share a dtype");
+  check_same_device(what, codes, scales, key_in, value_in, slot_mapping);
+  const c10::DeviceGuard guard(codes.device());
+  const int64_t num_blocks = codes.size(0), block = codes.size(2), heads = codes.size(3), d = 2 * codes.size(4);
+  auto by_head = [&](const Tensor& x) { return x.dim() == 2 && x.size(1) == heads * d ? x.unflatten(1, {heads, d}) : x; };
+  Tensor key = by_head(key_in), value = by_head(value_in);
+  TORCH_CHECK_VALUE(key.dim() == 3 && key.sizes() == value.sizes() && key.size(1) == heads && key.size(2) == d, what,
+                    ": key / value must be [num_tokens, num_kv_heads, head_size] matching the cache");
+  const int64_t num_tokens = key.size(0);
+  const Tensor slots = mx4_slots(what, slot_mapping, num_tokens);
+  if (num_tokens == 0) return;
+  key = aligned_rows(key);
+  value = aligned_rows(value);
+  check_rc(fxpr_reshape_and_cache_mx4(key.const_data_ptr(), value.const_data_ptr(), codes.mutable_data_ptr(),
+                                      scales.mutable_data_ptr(), code_of(t), slots.const_data_ptr<int64_t>(), num_tokens,
+                                      int(heads), int(d), int(block), num_blocks, key.stride(0), key.stride(1),
+                                      value.stride(0), value.stride(1), codes.stride(0), codes.stride(1),
+                                      codes.stride(2), codes.stride(3), scales.stride(0), scales.stride(1),
+                                      scales.stride(2), scales.stride(3), stream_of(codes)),
+           "fxpr_reshape_and_cache_mx4");
+}
+
+std::tuple<Tensor, Tensor> gather_cache_mx4(const Tensor& codes, const Tensor& scales, const Tensor& slot_mapping,
+                                            at::ScalarType out_dtype) {
+  const char* what = "gather_cache_mx4";
+  TORCH_CHECK(slot_mapping.is_cuda(), what, ": tensors must be CUDA");
+  check_mx4_cache(what, codes, scales);
+  TORCH_CHECK_TYPE(is_io(out_dtype), what, ": unsupported output dtype ", out_dtype,
+                   "; expected float16, bfloat16 or float32");
+  check_same_device(what, codes, scales, slot_mapping);
+  const c10::DeviceGuard guard(codes.device());
+  const Tensor slots = mx4_slots(what, slot_mapping, 0);
+  const int64_t n = slots.size(0), heads = codes.size(3), d = 2 * codes.size(4);
+  Tensor key = at::empty({n, heads, d}, codes.options().dtype(out_dtype)), value = at::empty_like(key);
+  if (key.numel())
+    check_rc(fxpr_gather_cache_mx4(codes.const_data_ptr(), scales.const_data_ptr(), key.mutable_data_ptr(),
+                                   value.mutable_data_ptr(), code_of(out_dtype), slots.const_data_ptr<int64_t>(), n,
+                                   int(heads), int(d), int(codes.size(2)), codes.size(0), codes.stride(0),
+                                   codes.stride(1), codes.stride(2), codes.stride(3), scales.stride(0),
+                                   scales.stride(1), scales.stride(2), scales.stride(3), stream_of(codes)),
+             "fxpr_gather_cache_mx4");
+  return {key, value};
+}
+
+void unified_attention_mx4(const Tensor& q_in, const Tensor& codes, const Tensor& scales, Tensor& o,
+                           const Tensor& query_start_loc, const Tensor& seq_lens, const Tensor& block_table,
+                           int64_t max_query_len, const std::optional<Tensor>& alibi_slopes, bool is_causal,
+                           std::optional<double> softmax_scale, int64_t int_bits, int64_t frac_bits,
+                           double logit_softcap, int64_t window_size, int64_t num_kv_splits) {
+  const char* what = "unified_attention_mx4_fxp";
+  check_int_bits(int_bits);
+  check_frac_bits(frac_bits);
+  TORCH_CHECK(q_in.is_cuda() && o.is_cuda() && query_start_loc.is_cuda() && seq_lens.is_cuda() && block_table.is_cuda(),
+              what, ": tensors must be CUDA");
+  check_mx4_cache(what, codes, scales);
+  const auto t = q_in.scalar_type();
+  TORCH_CHECK_TYPE(t == at::kHalf || t == at::kBFloat16, what, ": unsupported q dtype ", t,
+                   "; expected float16 or bfloat16");
+  TORCH_CHECK_TYPE(o.scalar_type() == t, what, ": o must share dtype with q");
+  TORCH_CHECK_TYPE(query_start_loc.scalar_type() == at::kInt, "query_start_loc must be int32");
+  TORCH_CHECK_TYPE(seq_lens.scalar_type() == at::kInt, "seq_lens must be int32");
+  TORCH_CHECK_TYPE(block_table.scalar_type() == at::kInt, "block_table must be int32");
+  TORCH_CHECK_VALUE(num_kv_splits >= 0, "num_kv_splits must be >= 0, got ", num_kv_splits);
+  const bool has_alibi = alibi_slopes.has_value() && alibi_slopes->defined() && alibi_slopes->numel() > 0;
+  TORCH_CHECK_TYPE(!has_alibi || alibi_slopes->scalar_type() == at::kFloat, "alibi_slopes must be float32");
+  check_same_device(what, q_in, codes, scales, o, query_start_loc, seq_lens, block_table);
+  TORCH_CHECK(!has_alibi || alibi_slopes->device() == q_in.device(), what, ": tensors must be on one device");
+
+  const c10::DeviceGuard guard(q_in.device());
+  const int64_t num_blocks = codes.size(0), page_size = codes.size(2), num_kv_heads = codes.size(3);
+  TORCH_CHECK_VALUE(q_in.dim() == 3, "q must be (num_tokens, num_heads, head_dim)");
+  const int64_t num_tokens = q_in.size(0), num_heads = q_in.size(1), head_dim = q_in.size(2);
+  TORCH_CHECK_VALUE(num_kv_heads != 0 && num_heads != 0 && num_heads % num_kv_heads == 0,
+                    "num_heads must be divisible by num_kv_heads");
+  TORCH_CHECK_VALUE(2 * codes.size(4) == head_dim && o.sizes() == q_in.sizes(),
+                    "q, o and the cache's head sizes must agree");
+  TORCH_CHECK_VALUE(page_size >= 16 && (page_size & (page_size - 1)) == 0, what,
+                    ": the cache's block_size must be a power of two, 16 or more, got ", page_size);
+  TORCH_CHECK_VALUE(!has_alibi || alibi_slopes->numel() == num_heads, "alibi_slopes must have one slope per head");
+  TORCH_CHECK_VALUE(seq_lens.dim() == 1 && query_start_loc.dim() == 1 && query_start_loc.size(0) == seq_lens.size(0) + 1,
+                    "query_start_loc must be 1-D with one more element than seq_lens");
+  const int64_t num_requests = seq_lens.size(0);
+  if (num_requests == 0 || num_tokens == 0) return;
+  TORCH_CHECK_VALUE(block_table.numel() % num_requests == 0 &&
+                        !(block_table.dim() == 2 && block_table.size(0) < num_requests),
+                    "block_table must have a row per request");
+  const Tensor q = aligned_rows(q_in);
+  Tensor out = o.stride(2) == 1 ? o : at::empty(o.sizes(), o.options());
+  Tensor bt = block_table.dim() == 2 ? block_table : block_table.reshape({num_requests, -1});
+  if (bt.stride(1) != 1) bt = bt.contiguous();
+  const Tensor qsl = query_start_loc.contiguous(), sl = seq_lens.contiguous();
+  const Tensor alibi = has_alibi ? alibi_slopes->contiguous() : Tensor();
+
+  constexpr double kRcpLn2 = 1.4426950408889634;
+  const double scale = softmax_scale.has_value() ? *softmax_scale : 1.0 / std::sqrt(double(head_dim));
+  const float softcap_log2 = logit_softcap > 0.0 ? float(logit_softcap * kRcpLn2) : 0.0f;
+  const int64_t max_blocks = bt.size(1), window = std::clamp<int64_t>(window_size, 0, 0x7fffffff);
+  const int64_t n = fxpr_attention_mx4_plan(int(num_requests), num_tokens, int(num_heads), int(num_kv_heads),
+                                            int(head_dim), int(page_size), int(max_query_len), int(max_blocks),
+                                            int(window), int(int_bits), int(num_kv_splits), nullptr);
+  Tensor ws = n > 0 ? bytes(n, q) : Tensor();
+  check_rc(fxpr_unified_attention_mx4(
+               q.const_data_ptr(), codes.const_data_ptr(), scales.const_data_ptr(), out.mutable_data_ptr(), code_of(t),
+               qsl.const_data_ptr<int32_t>(), sl.const_data_ptr<int32_t>(), bt.const_data_ptr<int32_t>(),
+               has_alibi ? alibi.const_data_ptr<float>() : nullptr, int(num_requests), num_tokens, int(num_heads),
+               int(num_kv_heads), int(head_dim), int(page_size), int(max_query_len), int(max_blocks), num_blocks,
+               q.stride(0), q.stride(1), codes.stride(0), codes.stride(1), codes.stride(2), codes.stride(3),
+               scales.stride(0), scales.stride(1), scales.stride(2), scales.stride(3), out.stride(0), out.stride(1),
+               bt.stride(0), is_causal ? 1 : 0, float(scale * kRcpLn2), softcap_log2, int(window), int(int_bits),
+               int(frac_bits), int(num_kv_splits), n > 0 ? ws.mutable_data_ptr() : nullptr, n, stream_of(q)),
+           "fxpr_unified_attention_mx4");
+  if (!out.is_same(o)) o.copy_(out);
+}
+
 }  // namespace
 
 // (set while the library is loaded: whether the launchers below were registered)
@@ -358,4 +518,7 @@ TORCH_LIBRARY_IMPL(fxpr, CUDA, m) {
   m.impl("gemm_fxp", &gemm);
   m.impl("unified_attention_fxp", &unified_attention);
   m.impl("reshape_and_cache", &reshape_and_cache);
+  m.impl("reshape_and_cache_mx4", &reshape_and_cache_mx4);
+  m.impl("gather_cache_mx4", &gather_cache_mx4);
+  m.impl("unified_attention_mx4_fxp", &unified_attention_mx4);
 }

@@ -54,6 +54,10 @@ SIGNATURES: dict[str, list] = {
     "fxpr_attention_splits": [_I, _I, _I, _I, _I, _I, _I],
     "fxpr_reshape_and_cache": [_P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _L,
                                _L, _L, _L, _L, _L, _L, _L, _L, _L, _L, _P],
+    "fxpr_reshape_and_cache_mx4": [_P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _L] + [_L] * 12 + [_P],
+    "fxpr_gather_cache_mx4": [_P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _L] + [_L] * 8 + [_P],
+    "fxpr_unified_attention_mx4": [_P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _L, _I, _I, _I, _I, _I, _I, _L] + [_L] * 13
+                                  + [_I, _F, _F, _I, _I, _I, _I, _P, _L, _P],
     # test hooks of the split log-softmax's bounded polls
     "fxpr_debug_set_lsm_spin_limit": [_I, _I],
     "fxpr_debug_lsm_default_spin_limit": [],
@@ -69,10 +73,11 @@ RESTYPES = {
                              ctypes.POINTER(ctypes.c_int32)], _L),
     "fxpr_attention_workspace_bytes": ([_I, _L, _I, _I, _I, _I, _I, _I, _I, _I], _L),
     "fxpr_sample_greedy_workspace_bytes": ([_L, _I], _L),
+    "fxpr_attention_mx4_plan": ([_I, _L, _I, _I, _I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(ctypes.c_int32)], _L),
 }
 
 # the ABI revision these signatures describe (include/fxpr.h, fxpr_abi_version)
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 _lib: ctypes.CDLL | None = None
 _lock = threading.Lock()

@@ -2,14 +2,15 @@
 
 The six reference schemas are kept verbatim (fxpr_vllm/_lib.py:13-33 of the
 reference) so callers and torch.compile graphs are a drop-in; PyTorch-ROCm
-dispatches HIP tensors through the CUDA key. Nine schemas are new in this
+dispatches HIP tensors through the CUDA key. Twelve schemas are new in this
 build: the shard halves of gemm_fxp and log_softmax_fxp for more than one
 device (below), fixed_row_sum (the integer sum the reference's tests do with torch,
 _tests/test_sum.py:12-16), log_softmax_fxp (listed in the reference
 README.md:60 but not shipped), sample_greedy_fxp (the sampler of the
 reference's README.md:69, likewise not shipped) and reshape_and_cache (the
 KV-cache write the reference backend takes from vLLM,
-attention_backend.py:253-277). Validation and error classes follow the
+attention_backend.py:253-277), and the KV cache in 4 bits: its write, its read
+back and the attention over it. Validation and error classes follow the
 reference impls (_lib.py:36-129).
 """
 
@@ -25,6 +26,7 @@ from ._kernels import attention as _attention
 from ._kernels import cache as _cache
 from ._kernels import casts as _casts
 from ._kernels import gemm as _gemm
+from ._kernels import mx4 as _mx4
 from ._kernels import rows as _rows
 from ._kernels import sampling as _sampling
 
@@ -63,6 +65,21 @@ _lib.define(
 _lib.define(
     "sample_greedy_fxp(Tensor logits, int num_logprobs, int fxp_int_bits, "
     "int fxp_frac_bits) -> (Tensor, Tensor, Tensor, Tensor)"
+)
+# The KV cache in 4 bits: codes [num_blocks, 2, block_size, num_kv_heads, head_size / 2]
+# and scales [..., head_size / 32], uint8 (format: include/fxpr.h).
+_lib.define(
+    "reshape_and_cache_mx4(Tensor key, Tensor value, Tensor(a!) kv_codes, Tensor(b!) kv_scales, "
+    "Tensor slot_mapping) -> ()"
+)
+_lib.define(
+    "gather_cache_mx4(Tensor kv_codes, Tensor kv_scales, Tensor slot_mapping, ScalarType out_dtype) -> (Tensor, Tensor)"
+)
+_lib.define(
+    "unified_attention_mx4_fxp(Tensor q, Tensor kv_codes, Tensor kv_scales, Tensor(a!) o, "
+    "Tensor query_start_loc, Tensor seq_lens, Tensor block_table, int max_query_len, "
+    "Tensor? alibi_slopes, bool is_causal, float? softmax_scale, int fxp_int_bits, int fxp_frac_bits, "
+    "float logit_softcap, int window_size, int num_kv_splits) -> ()"
 )
 # Shard halves for more than one device: a K-sharded (row-parallel) GEMM's
 # integer accumulators and their epilogue; a vocab-sharded log-softmax's row
@@ -160,6 +177,28 @@ def _sample_greedy_fxp_cuda(logits: torch.Tensor, num_logprobs: int, fxp_int_bit
     return _sampling.sample_greedy_fxp_run(logits, int(num_logprobs), int(fxp_int_bits), int(fxp_frac_bits))
 
 
+def _reshape_and_cache_mx4_cuda(key: torch.Tensor, value: torch.Tensor, kv_codes: torch.Tensor,
+                                kv_scales: torch.Tensor, slot_mapping: torch.Tensor):
+    _mx4.reshape_and_cache_run(key, value, kv_codes, kv_scales, slot_mapping)
+
+
+def _gather_cache_mx4_cuda(kv_codes: torch.Tensor, kv_scales: torch.Tensor, slot_mapping: torch.Tensor,
+                           out_dtype: torch.dtype):
+    return _mx4.gather_cache_run(kv_codes, kv_scales, slot_mapping, out_dtype)
+
+
+def _unified_attention_mx4_fxp_cuda(q, kv_codes, kv_scales, o, query_start_loc, seq_lens, block_table, max_query_len,
+                                    alibi_slopes, is_causal, softmax_scale, fxp_int_bits, fxp_frac_bits, logit_softcap,
+                                    window_size, num_kv_splits):
+    _check_int_bits(fxp_int_bits)
+    _check_frac_bits(fxp_frac_bits)
+    _mx4.unified_attention_run(
+        q, kv_codes, kv_scales, o, query_start_loc, seq_lens, block_table, int(max_query_len), alibi_slopes,
+        bool(is_causal), None if softmax_scale is None else float(softmax_scale), int(fxp_int_bits), int(fxp_frac_bits),
+        float(logit_softcap), int(window_size), int(num_kv_splits),
+    )
+
+
 def _gemm_fxp_partial_cuda(a, b, fxp_int_bits, fxp_frac_bits):
     _check_int_bits(fxp_int_bits)
     _check_frac_bits(fxp_frac_bits)
@@ -227,6 +266,9 @@ _WITH_NATIVE = {
     "log_softmax_fxp": _log_softmax_fxp_cuda,
     "reshape_and_cache": _reshape_and_cache_cuda,
     "sample_greedy_fxp": _sample_greedy_fxp_cuda,
+    "reshape_and_cache_mx4": _reshape_and_cache_mx4_cuda,
+    "gather_cache_mx4": _gather_cache_mx4_cuda,
+    "unified_attention_mx4_fxp": _unified_attention_mx4_fxp_cuda,
 }
 for _name, _fn in _WITH_NATIVE.items():
     if not _NATIVE:

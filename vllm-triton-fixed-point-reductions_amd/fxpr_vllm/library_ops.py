@@ -88,6 +88,24 @@ def _reshape_and_cache_fake(key, value, kv_cache, slot_mapping):
     return None
 
 
+@torch.library.register_fake("fxpr::reshape_and_cache_mx4")
+def _reshape_and_cache_mx4_fake(key, value, kv_codes, kv_scales, slot_mapping):
+    return None
+
+
+@torch.library.register_fake("fxpr::gather_cache_mx4")
+def _gather_cache_mx4_fake(kv_codes, kv_scales, slot_mapping, out_dtype):
+    shape = (slot_mapping.shape[0], kv_codes.shape[3], 2 * kv_codes.shape[4])
+    return kv_codes.new_empty(shape, dtype=out_dtype), kv_codes.new_empty(shape, dtype=out_dtype)
+
+
+@torch.library.register_fake("fxpr::unified_attention_mx4_fxp")
+def _unified_attention_mx4_fxp_fake(q, kv_codes, kv_scales, o, query_start_loc, seq_lens, block_table, max_query_len,
+                                    alibi_slopes, is_causal, softmax_scale, fxp_int_bits, fxp_frac_bits, logit_softcap,
+                                    window_size, num_kv_splits):
+    return None
+
+
 @torch.library.register_fake("fxpr::gemm_fxp_partial")
 def _gemm_fxp_partial_fake(a, b, fxp_int_bits, fxp_frac_bits):
     return a.new_empty((a.shape[0], b.shape[1]), dtype=torch.int64 if int(fxp_int_bits) == 64 else torch.int32)
@@ -126,5 +144,8 @@ fixed_to_float = torch.ops.fxpr.fixed_to_float
 fixed_row_sum = torch.ops.fxpr.fixed_row_sum
 log_softmax_fxp = torch.ops.fxpr.log_softmax_fxp
 reshape_and_cache = torch.ops.fxpr.reshape_and_cache
+reshape_and_cache_mx4 = torch.ops.fxpr.reshape_and_cache_mx4
+gather_cache_mx4 = torch.ops.fxpr.gather_cache_mx4
+unified_attention_mx4_fxp = torch.ops.fxpr.unified_attention_mx4_fxp
 sample_greedy_fxp = torch.ops.fxpr.sample_greedy_fxp
 unified_attention_fxp = torch.ops.fxpr.unified_attention_fxp
