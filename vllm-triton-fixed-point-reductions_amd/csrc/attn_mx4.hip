@@ -133,8 +133,14 @@ extern "C" int fxpr_unified_attention_mx4(
   const int64_t max_rows = int64_t(max_query_len > 1 ? max_query_len : 1) * (num_heads / num_kv_heads);
   Planned plan = plan_mx4(num_requests, num_tokens, num_heads, num_kv_heads, head_dim, page_size, max_query_len,
                           max_blocks_per_seq, std::max(window_size, 0), int_bits, num_kv_splits);
+  // (quotient()'s ranges: rows of a request by the group, request x kv head by
+  // the kv heads)
+  const int64_t group = num_heads / num_kv_heads;
+  if ((std::max(max_rows, num_tokens * group) + 64 * (int64_t(num_requests) + 1)) * group > int64_t(0xffffffff) ||
+      int64_t(num_requests) * num_kv_heads * num_kv_heads > int64_t(0xffffffff))
+    return FXPR_E_SHAPE;
   if (max_rows > int64_t(0x7fffffff) ||
-      (num_tokens * (num_heads / num_kv_heads) / PQROWS + num_requests) * num_kv_heads > int64_t(0x7fffffff))
+      (num_tokens * group / PQROWS + num_requests) * num_kv_heads > int64_t(0x7fffffff))
     return FXPR_E_SHAPE;
   if (plan.ws.total > 0 && (!workspace || workspace_bytes < plan.ws.total)) return FXPR_E_WORKSPACE;
 
@@ -150,6 +156,8 @@ extern "C" int fxpr_unified_attention_mx4(
   m.s_blk = uint32_t(stride_scales_block);
   m.s_slot = uint32_t(stride_scales_slot);
   m.s_head = uint32_t(stride_scales_head);
+  m.by_group = reciprocal(uint32_t(num_heads / num_kv_heads));
+  m.by_heads = reciprocal(uint32_t(num_kv_heads));
   a.q = q;
   a.o = o;
   a.qsl = query_start_loc;

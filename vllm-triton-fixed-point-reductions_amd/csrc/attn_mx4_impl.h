@@ -36,7 +36,41 @@ struct Mx4Args {
   const uint8_t* ks;
   const uint8_t* vs;
   uint32_t c_blk, c_slot, c_head, s_blk, s_slot, s_head;  // bytes
+  uint32_t by_group, by_heads;  // ceil(2^32 / x): x / group and x / num_kv_heads by a high product (see quotient)
 };
+
+// x / d with m = ceil(2^32 / d): exact while x d < 2^32 (the excess of m over
+// 2^32 / d is below 1, so the product is off by less than x / 2^32, and x / d is
+// at least 1 / d from the next integer). The host checks the ranges; d = 1 has
+// m = 0. (An integer division by a variable is some 30 instructions, and a
+// decode workgroup has only 8 key tiles to spread its start over.)
+__host__ __device__ __forceinline__ uint32_t reciprocal(uint32_t d) {
+  return d <= 1 ? 0u : uint32_t(((uint64_t(1) << 32) + d - 1) / d);
+}
+__device__ __forceinline__ uint32_t quotient(uint32_t x, uint32_t m) { return m == 0 ? x : __umulhi(x, m); }
+
+// row_info (attn_impl.h) by quotient().
+__device__ __forceinline__ RowInfo row_at(const Mx4Args& m, int g, int q_start, int q_len, int ctx, int seq_len, int row) {
+  const AttnArgs& a = m.a;
+  RowInfo ri;
+  const int rows_total = q_len * a.group;
+  const int rr = row < rows_total ? row : 0;
+  const int i = int(quotient(uint32_t(rr), m.by_group));
+  ri.token = q_start + i;
+  ri.valid = row < rows_total && ri.token >= 0 && ri.token < a.num_tokens;
+  if (!ri.valid) ri.token = 0;
+  ri.head = g * a.group + (rr - i * a.group);
+  ri.qpos = ctx + i;
+  ri.kend = a.causal ? min(seq_len, ri.qpos + 1) : seq_len;
+  ri.kstart = a.window > 0 ? max(0, ri.qpos - a.window + 1) : 0;
+  return ri;
+}
+
+// The rounding constant of the fast quantisation: for |x| 2^f < 2^22,
+// fl(x 2^f + 1.5 2^23) (exact product, one rounding, spacing 1, an even
+// constant) has the bits of RNE(x 2^f) + kRound.
+constexpr float kRoundF = 12582912.0f;
+constexpr uint32_t kRound = 0x4B400000u;
 
 // Host plan of a launch.
 struct Mx4Plan {
@@ -134,6 +168,12 @@ struct Pager {
   __device__ __forceinline__ uint64_t offset(int g, int e, uint32_t blk, uint32_t slot, uint32_t head_off) const {
     return uint64_t(block(e)) * blk + uint64_t(uint32_t((16 * g) & page_mask)) * slot + head_off;
   }
+  // the largest row offset (row index times slot) within granule g that lies in
+  // the sequence: a lane takes the smaller of its own and this, so rows past the
+  // sequence read bytes of its last row (their keys are masked)
+  __device__ __forceinline__ uint32_t limit(int g, uint32_t slot) const {
+    return uint32_t(min(last_key - 16 * g, 15)) * slot;
+  }
 };
 
 template <class A> __device__ __forceinline__ Pager make_pager(const A& a, int r, int seq_len) {
@@ -155,8 +195,13 @@ template <class A> __device__ __forceinline__ Pager make_pager(const A& a, int r
 // added in any order to the same bits (attn_impl.h's waves split them by d
 // instead). Loads run a phase ahead: a chunk's V goes out before its scores,
 // the next chunk's K before the weights.
-template <int DT, int BITS, int D, bool SPLIT>
-__global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn_mx4_rows16_kernel(Mx4Args m) {
+//
+// FAST (the same bits): no softcap or ALiBi and a positive scale, so a score is
+// fl(dot * scale) and the chunk maximum fl(max(dot) * scale); sums by the
+// rounding constant (a weight is at most 1; a tile whose weighted V leaves the
+// constant's range is added exactly).
+template <int DT, int BITS, int D, bool SPLIT, bool FAST>
+__device__ __forceinline__ void rows16_body(const Mx4Args& m) {
   const AttnArgs& a = m.a;
   using TR = Traits<DT>;
   using T = typename TR::T;
@@ -167,6 +212,7 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
   constexpr int STAGEB = 32 * L::ROWB;             // the wave's V stage
   constexpr int PARTB = QROWS * D * int(sizeof(AccT));  // the wave's partial sums, in the stage's place
   constexpr int WAVEB = STAGEB > PARTB ? STAGEB : PARTB;
+  constexpr int EPC = 16 / int(sizeof(AccT));      // partial sums per 16-byte chunk
   __shared__ __align__(16) unsigned char stage_all[4 * WAVEB];
   __shared__ float red_m[2][4][QROWS];  // (by the chunk's parity: no third barrier)
   __shared__ AccT red_d[4][QROWS];
@@ -174,7 +220,7 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
   const int tid = threadIdx.x, lane = tid & 63, kg = lane >> 4, i16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   unsigned char* stage = stage_all + wave * WAVEB;
-  const int r = blockIdx.x / a.num_kv_heads, g = blockIdx.x % a.num_kv_heads;
+  const int r = int(quotient(blockIdx.x, m.by_heads)), g = int(blockIdx.x) - r * a.num_kv_heads;
   const int split = blockIdx.z;
   const int q_start = ((ConstI32)a.qsl)[r];
   const int q_len = ((ConstI32)a.qsl)[r + 1] - q_start;
@@ -186,8 +232,8 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
   if (a.pq_rows > 0 && rows_total >= a.pq_rows) return;  // attn_mx4_rows64_kernel's request
   auto ws_row = [&](int64_t token) { return a.tok_cap > 0 ? int64_t(r) * a.tok_cap + (token - q_start) : token; };
 
-  const int i_min = row0 / a.group;
-  const int i_max = min(rows_total - 1, row0 + QROWS - 1) / a.group;
+  const int i_min = int(quotient(uint32_t(row0), m.by_group));
+  const int i_max = int(quotient(uint32_t(min(rows_total - 1, row0 + QROWS - 1)), m.by_group));
   const int hi = a.causal ? min(seq_len, ctx + i_max + 1) : seq_len;
   const int lo = a.window > 0 ? max(0, ctx + i_min - a.window + 1) : 0;
   const int t_lo = lo / TILE;
@@ -201,7 +247,7 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
   const int c_hi = min(c_first + nch, c_lo + per);
 
   // the thread's part of the sums: row tid / 16, elements VPT (tid % 16) ..
-  const RowInfo mine = row_info(a, g, q_start, q_len, ctx, seq_len, row0 + (tid >> 4));
+  const RowInfo mine = row_at(m, g, q_start, q_len, ctx, seq_len, row0 + (tid >> 4));
   const int my_d = VPT * (tid & 15);
   if (SPLIT && split == 0 && (tid & 15) == 0 && mine.valid) {
     int* cr = a.crange + 2 * (ws_row(mine.token) * a.num_heads + mine.head);
@@ -212,20 +258,6 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
 
   const Pager pager = make_pager(a, r, seq_len);
   const uint32_t ch = uint32_t(g) * m.c_head, sh = uint32_t(g) * m.s_head;
-
-  // The lane's query row (a column of the score MFMAs).
-  const RowInfo me = row_info(a, g, q_start, q_len, ctx, seq_len, row0 + i16);
-  u32x4 qf[QS];
-  {
-    const T* qbase = static_cast<const T*>(a.q) + me.token * a.sq_t + int64_t(me.head) * a.sq_h;
-#pragma unroll
-    for (int j = 0; j < QS; ++j)
-      qf[j] = me.valid ? *reinterpret_cast<const u32x4*>(qbase + 32 * j + 8 * kg) : u32x4{0u, 0u, 0u, 0u};
-  }
-  const int ks = me.valid ? me.kstart : 0x7fffffff;
-  const int ke = me.valid ? me.kend : 0;
-  const int qp = me.qpos;
-  const float slope = a.alibi ? a.alibi[me.head] : 0.0f;
 
   auto live_lo = [&](int c) { return max(c * CT, t_lo); };
   auto live_hi = [&](int c) { return min(c * CT + CT, t_hi); };
@@ -242,7 +274,17 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
   };
 
   // K: MFMA row i16 of (s, h) is the tile's key 32 s + pi(i16, h), in granule
-  // 2 s + i16 / 8.
+  // 2 s + i16 / 8. (Offsets within a granule with the limits of Pager; a code
+  // offset holds the lane's unit too, and its limit the last unit.)
+  const bool up = i16 >= 8;
+  uint32_t kc_off[2], ks_off[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t in = uint32_t((8 * (i16 >> 2) + 4 * h + (i16 & 3)) & 15);
+    kc_off[h] = in * m.c_slot + kg * (D / 8);
+    ks_off[h] = in * m.s_slot;
+  }
+  constexpr uint32_t kLastUnit = 3 * (D / 8);
   Units<D> kb[NT][4];
   Scales<D> kbs[NT][4];
   auto load_k = [&](int c) __attribute__((always_inline)) {
@@ -256,20 +298,20 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
         const uint64_t c1 = pager.offset(g1, ent[u][2 * s + 1], m.c_blk, m.c_slot, ch);
         const uint64_t s0 = pager.offset(g0, ent[u][2 * s], m.s_blk, m.s_slot, sh);
         const uint64_t s1 = pager.offset(g1, ent[u][2 * s + 1], m.s_blk, m.s_slot, sh);
-        const bool up = i16 >= 8;
-        const uint8_t* cp = m.kc + (up ? c1 : c0) + kg * (D / 8);
-        const uint8_t* sp = m.ks + (up ? s1 : s0);
+        const uint8_t* cp = up ? m.kc + c1 : m.kc + c0;
+        const uint8_t* sp = up ? m.ks + s1 : m.ks + s0;
+        const uint32_t cl = (up ? pager.limit(g1, m.c_slot) : pager.limit(g0, m.c_slot)) + kLastUnit;
+        const uint32_t sl = up ? pager.limit(g1, m.s_slot) : pager.limit(g0, m.s_slot);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int key = t * TILE + 32 * s + 8 * (i16 >> 2) + 4 * h + (i16 & 3);
-          const uint32_t in = uint32_t(min(key, pager.last_key) - 16 * (up ? g1 : g0));
-          kb[u][2 * s + h] = load_units<D>(cp + in * m.c_slot);
-          kbs[u][2 * s + h] = load_scales<D>(sp + in * m.s_slot);
+          kb[u][2 * s + h] = load_units<D>(cp + min(kc_off[h], cl));
+          kbs[u][2 * s + h] = load_scales<D>(sp + min(ks_off[h], sl));
         }
       }
     }
   };
   // V: lane l of load q has row 16 q + l / 4 of the tile, units l % 4.
+  const uint32_t vc_off = uint32_t(lane >> 2) * m.c_slot + (lane & 3) * (D / 8), vs_off = uint32_t(lane >> 2) * m.s_slot;
   Units<D> vb[NT][4];
   Scales<D> vbs[NT][4];
   auto load_v = [&](int c) __attribute__((always_inline)) {
@@ -281,19 +323,43 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
         const int gq = pager.granule(4 * t + q);
         const uint8_t* cp = m.vc + pager.offset(gq, ent[u][q], m.c_blk, m.c_slot, ch);
         const uint8_t* sp = m.vs + pager.offset(gq, ent[u][q], m.s_blk, m.s_slot, sh);
-        const int key = t * TILE + 16 * q + (lane >> 2);
-        const uint32_t in = uint32_t(min(key, pager.last_key) - 16 * gq);
-        vb[u][q] = load_units<D>(cp + (in * m.c_slot + (lane & 3) * (D / 8)));
-        vbs[u][q] = load_scales<D>(sp + in * m.s_slot);
+        vb[u][q] = load_units<D>(cp + min(vc_off, pager.limit(gq, m.c_slot) + kLastUnit));
+        vbs[u][q] = load_scales<D>(sp + min(vs_off, pager.limit(gq, m.s_slot)));
       }
     }
   };
+  if (c_lo < c_hi) {
+    load_entries(c_lo);
+    load_k(c_lo);
+  }
 
-  // LDS addresses of the V stage: the row and chunk slots the lane writes, and
-  // its transposing reads (keys 8 kg + j / 4 + 4 h, columns 4 (j % 4) of d block
-  // 0; d block db is at ^ (db << 5)).
-  const int wr = lane >> 2;
-  unsigned vrd[2];
+  // The lane's query row (a column of the score MFMAs).
+  const RowInfo me = row_at(m, g, q_start, q_len, ctx, seq_len, row0 + i16);
+  u32x4 qf[QS];
+  {
+    const T* qbase = static_cast<const T*>(a.q) + me.token * a.sq_t + int64_t(me.head) * a.sq_h;
+#pragma unroll
+    for (int j = 0; j < QS; ++j)
+      qf[j] = me.valid ? *reinterpret_cast<const u32x4*>(qbase + 32 * j + 8 * kg) : u32x4{0u, 0u, 0u, 0u};
+  }
+  const int ks = me.valid ? me.kstart : 0x7fffffff;
+  const int ke = me.valid ? me.kend : 0;
+  const int qp = me.qpos;
+  const float slope = !FAST && a.alibi ? a.alibi[me.head] : 0.0f;
+  // (rows outside the request see no key and are never stored: a tile counts as
+  // whole when every row of the request sees all of it)
+  auto tile_whole = [&](int t) -> bool {
+    return __builtin_amdgcn_ballot_w64(me.valid && !(ks <= t * TILE && t * TILE + TILE <= ke)) == 0;
+  };
+
+  // LDS addresses of the V stage: the chunk slots the lane writes (row lane / 4;
+  // the second granule is 16 rows on, which the swizzle ignores), and its
+  // transposing reads (keys 8 kg + j / 4 + 4 h, columns 4 (j % 4) of d block 0;
+  // d block db is at ^ (db << 5)).
+  unsigned vwr[QS], vrd[2];
+#pragma unroll
+  for (int j = 0; j < QS; ++j)
+    vwr[j] = (lane >> 2) * L::ROWB + (((4 * j + (lane & 3)) ^ L::vswz(lane >> 2)) << 4);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int rr = 8 * kg + (i16 >> 2) + 4 * h;
@@ -304,17 +370,17 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
   AccT Dn = 0, W[VPT];
 #pragma unroll
   for (int v = 0; v < VPT; ++v) W[v] = 0;
+  [[maybe_unused]] const float vlim = (BITS == 16 ? 32767.0f : 4194304.0f) / a.fxp_scale;
 
   if (c_lo < c_hi) {
-    load_entries(c_lo);
-    load_k(c_lo);
     for (int c = c_lo;; ++c) {
       const int ta = live_lo(c), te = live_hi(c);
       load_v(c);
       if (c + 1 < c_hi) load_entries(c + 1);
 
-      // scores of the wave's tiles, for the lane's row and keys 32 s + 8 kg + 4 h + e
-      float sc[NT][4][4];
+      // the wave's tiles: dots (FAST) or scores, for the lane's row and keys
+      // 32 s + 8 kg + 4 h + e, -inf where masked
+      f32x4 sc[NT][4];
       float mx = -__builtin_inff();
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
@@ -326,29 +392,45 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
 #pragma unroll
           for (int j = 0; j < QS; ++j)
             acc = TR::mma(mx4::unpack8<DT>(kb[u][q].w[j], mx4::scale_of<DT>(kbs[u][q].w[j / 4], j % 4)), qf[j], acc);
-          const int key0 = t * TILE + 32 * (q >> 1) + 8 * kg + 4 * (q & 1);
+          if constexpr (!FAST) {
+            const int key0 = t * TILE + 32 * (q >> 1) + 8 * kg + 4 * (q & 1);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = __fmul_rn(acc[e], a.scale_log2);
-            if (a.softcap_log2 > 0.0f) x = softcapped(x, a.softcap_log2);
-            if (a.alibi) x = x + slope * static_cast<float>(key0 + e - qp);
-            sc[u][q][e] = (live && key0 + e >= ks && key0 + e < ke) ? x : -__builtin_inff();
-            mx = fmaxf(mx, sc[u][q][e]);
+            for (int e = 0; e < 4; ++e) {
+              float x = __fmul_rn(acc[e], a.scale_log2);
+              if (a.softcap_log2 > 0.0f) x = softcapped(x, a.softcap_log2);
+              if (a.alibi) x = x + slope * static_cast<float>(key0 + e - qp);
+              acc[e] = x;
+            }
           }
+          sc[u][q] = acc;
         }
+        if (!live || !tile_whole(t)) {  // uniform
+          const int k0 = t * TILE + 8 * kg;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = k0 + 32 * (q >> 1) + 4 * (q & 1) + e;
+              sc[u][q][e] = (live && key >= ks && key < ke) ? sc[u][q][e] : -__builtin_inff();
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mx = fmaxf(fmaxf(mx, fmaxf(sc[u][q][0], sc[u][q][1])), fmaxf(sc[u][q][2], sc[u][q][3]));
       }
       if (c + 1 < c_hi) load_k(c + 1);
 
       // the chunk's row maxima: the row's four lanes, then the waves
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      if constexpr (FAST) mx = __fmul_rn(mx, a.scale_log2);
       float(&rm)[4][QROWS] = red_m[c & 1];
       if (kg == 0) rm[wave][i16] = mx;
       lds_barrier();
       mx = fmaxf(fmaxf(rm[0][i16], rm[1][i16]), fmaxf(rm[2][i16], rm[3][i16]));
       const float mrow = mx != -__builtin_inff() ? mx : 0.0f;  // no key: pin to 0
 
-      // weights and weighted V of the wave's tiles
+      // weights and weighted V of the wave's tiles. FAST: the sums carry
+      // kRound per added term, taken out below.
       AccT den = 0;
       AccT wv[DBLK][4];
 #pragma unroll
@@ -367,27 +449,37 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
             u32x4 pb;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              uint32_t p16[4];
+              float w[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float w = __builtin_amdgcn_exp2f(sc[u][2 * s + h][e] - mrow);
-                den = wadd<BITS>(den, quant<BITS>(__fmul_rn(w, a.fxp_scale)));
-                p16[e] = Io<DT>::store(w);
+                const float x = FAST ? __fmul_rn(sc[u][2 * s + h][e], a.scale_log2) : sc[u][2 * s + h][e];
+                w[e] = __builtin_amdgcn_exp2f(x - mrow);
               }
-              pb[2 * h] = p16[0] | (p16[1] << 16);
-              pb[2 * h + 1] = p16[2] | (p16[3] << 16);
+              if constexpr (FAST) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)  // (the maximum: NaN counts as 0)
+                  den = AccT(uint32_t(den) + __float_as_uint(fmaxf(__builtin_fmaf(w[e], a.fxp_scale, kRoundF), kRoundF)));
+                pb[2 * h] = p_pack2<DT>(w[0], w[1]);
+                pb[2 * h + 1] = p_pack2<DT>(w[2], w[3]);
+              } else {
+                uint32_t p16[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  den = wadd<BITS>(den, quant<BITS>(__fmul_rn(w[e], a.fxp_scale)));
+                  p16[e] = Io<DT>::store(w[e]);
+                }
+                pb[2 * h] = p16[0] | (p16[1] << 16);
+                pb[2 * h + 1] = p16[2] | (p16[3] << 16);
+              }
             }
             lds_wave_order();
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int rr = 16 * q + wr;
-              unsigned char* row = stage + rr * L::ROWB;
+            for (int q = 0; q < 2; ++q)
 #pragma unroll
               for (int j = 0; j < QS; ++j)
-                lds_store16(row + (((4 * j + (lane & 3)) ^ L::vswz(rr)) << 4),
+                lds_store16(stage + vwr[j] + q * 16 * L::ROWB,
                             mx4::unpack8<DT>(vb[u][2 * s + q].w[j],
                                              mx4::scale_of<DT>(vbs[u][2 * s + q].w[j / 4], j % 4)));
-            }
             lds_wave_order();
 #pragma unroll
             for (int b = 0; b < DBLK; ++b) {
@@ -396,47 +488,89 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
               acc[b] = TR::mma(u32x4{lo2[0], lo2[1], hi2[0], hi2[1]}, pb, acc[b]);
             }
           }
+          if constexpr (FAST) {
+            den = AccT(uint32_t(den) - 16u * kRound);
+            float vmax = 0.0f;
 #pragma unroll
-          for (int b = 0; b < DBLK; ++b)
+            for (int b = 0; b < DBLK; ++b) {
+              vmax = absmax4(vmax, acc[b]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) wv[b][e] = wadd<BITS>(wv[b][e], quant<BITS>(__fmul_rn(acc[b][e], a.fxp_scale)));
+              for (int e = 0; e < 4; ++e)
+                wv[b][e] = AccT(uint32_t(wv[b][e]) + __float_as_uint(__builtin_fmaf(acc[b][e], a.fxp_scale, kRoundF)));
+            }
+            if (__builtin_amdgcn_ballot_w64(!(vmax < vlim)) != 0) {  // uniform: out of the constant's range
+#pragma unroll
+              for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t without =
+                      uint32_t(wv[b][e]) - __float_as_uint(__builtin_fmaf(acc[b][e], a.fxp_scale, kRoundF));
+                  wv[b][e] = AccT(uint32_t(wadd<BITS>(AccT(without), quant<BITS>(__fmul_rn(acc[b][e], a.fxp_scale)))) + kRound);
+                }
+            }
+          } else {
+#pragma unroll
+            for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                wv[b][e] = wadd<BITS>(wv[b][e], quant<BITS>(__fmul_rn(acc[b][e], a.fxp_scale)));
+          }
         }
       }
 
-      // the waves' partial sums to LDS: lane (kg, row) holds d = 16 b + 4 kg + e
+      // the waves' partial sums to LDS, rows of D with 16-byte chunk x of row i
+      // at x ^ i: lane (kg, row) holds d = 16 b + 4 kg + e
       den = wadd<BITS>(den, __shfl_xor(den, 16, 64));
       den = wadd<BITS>(den, __shfl_xor(den, 32, 64));
       if (kg == 0) red_d[wave][i16] = den;
       lds_wave_order();
-      {
-        typedef AccT acc4 __attribute__((ext_vector_type(4)));
-        acc4* p = reinterpret_cast<acc4*>(stage) + i16 * (D / 4);
+      if (me.valid) {
+        typedef AccT accc __attribute__((ext_vector_type(EPC)));
+        accc* p = reinterpret_cast<accc*>(stage) + i16 * (D / EPC);
 #pragma unroll
-        for (int b = 0; b < DBLK; ++b) p[4 * b + kg] = acc4{wv[b][0], wv[b][1], wv[b][2], wv[b][3]};
+        for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+          for (int x = 0; x < 4 / EPC; ++x) {
+            accc v;
+#pragma unroll
+            for (int e = 0; e < EPC; ++e) v[e] = wv[b][x * EPC + e];
+            p[((4 * b + kg) * (4 / EPC) + x) ^ i16] = v;
+          }
       }
       lds_barrier();
-      {
+      if (mine.valid) {
+        typedef AccT accc __attribute__((ext_vector_type(EPC)));
         const int row = tid >> 4;
-        AccT cd = wadd<BITS>(wadd<BITS>(red_d[0][row], red_d[1][row]), wadd<BITS>(red_d[2][row], red_d[3][row]));
+        const AccT cd = wadd<BITS>(wadd<BITS>(red_d[0][row], red_d[1][row]), wadd<BITS>(red_d[2][row], red_d[3][row]));
         const float cm = fmaxf(fmaxf(rm[0][row], rm[1][row]), fmaxf(rm[2][row], rm[3][row]));
         AccT cw[VPT];
 #pragma unroll
-        for (int v = 0; v < VPT; ++v) {
-          cw[v] = 0;
+        for (int x = 0; x < VPT / EPC; ++x) {
+          const int at = row * (D / EPC) + ((my_d / EPC + x) ^ row);
+          accc v[4];
 #pragma unroll
-          for (int w = 0; w < 4; ++w)
-            cw[v] = wadd<BITS>(cw[v], reinterpret_cast<const AccT*>(stage_all + w * WAVEB)[row * D + my_d + v]);
+          for (int w = 0; w < 4; ++w) v[w] = reinterpret_cast<const accc*>(stage_all + w * WAVEB)[at];
+#pragma unroll
+          for (int e = 0; e < EPC; ++e)
+            cw[x * EPC + e] = wadd<BITS>(wadd<BITS>(v[0][e], v[1][e]), wadd<BITS>(v[2][e], v[3][e]));
+        }
+        if constexpr (FAST) {
+#pragma unroll
+          for (int v = 0; v < VPT; ++v) cw[v] = AccT(uint32_t(cw[v]) - uint32_t(te - ta) * kRound);
         }
         if constexpr (SPLIT) {
-          if (mine.valid) {
-            const int64_t slot = (ws_row(mine.token) * a.num_heads + mine.head) * a.chunk_slots + c;
-            if ((tid & 15) == 0) {
-              a.pmax[slot] = cm;
-              static_cast<AccT*>(a.den_ws)[slot] = cd;
-            }
-            AccT* wp = static_cast<AccT*>(a.wv_ws) + slot * D + my_d;
+          const int64_t slot = (ws_row(mine.token) * a.num_heads + mine.head) * a.chunk_slots + c;
+          if ((tid & 15) == 0) {
+            a.pmax[slot] = cm;
+            static_cast<AccT*>(a.den_ws)[slot] = cd;
+          }
+          AccT* wp = static_cast<AccT*>(a.wv_ws) + slot * D + my_d;
 #pragma unroll
-            for (int v = 0; v < VPT; ++v) wp[v] = cw[v];
+          for (int x = 0; x < VPT / EPC; ++x) {
+            accc v;
+#pragma unroll
+            for (int e = 0; e < EPC; ++e) v[e] = cw[x * EPC + e];
+            reinterpret_cast<accc*>(wp)[x] = v;
           }
         } else if (cm != -__builtin_inff()) {
           float Mn, fa, fb;
@@ -461,6 +595,11 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
       for (int v = 0; v < VPT; ++v) o[v] = Io<DT>::store(div_rn(acc_f32<BITS>(W[v], a.fxp_inv), den_f));
     }
   }
+}
+
+template <int DT, int BITS, int D, bool SPLIT, bool FAST>
+__global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn_mx4_rows16_kernel(Mx4Args m) {
+  rows16_body<DT, BITS, D, SPLIT, FAST>(m);
 }
 
 // ---------------------------------------------------------------------------
@@ -521,7 +660,7 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
   const uint32_t ch = uint32_t(g) * m.c_head, sh = uint32_t(g) * m.s_head;
 
   // The lane's query row.
-  const RowInfo me = row_info(a, g, q_start, q_len, ctx, seq_len, wrow0 + i16);
+  const RowInfo me = row_at(m, g, q_start, q_len, ctx, seq_len, wrow0 + i16);
   u32x4 qf[QS];
   {
     const T* qbase = static_cast<const T*>(a.q) + me.token * a.sq_t + int64_t(me.head) * a.sq_h;
@@ -541,15 +680,15 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
     Scales<D> s;
   };
   const int srow = 16 * wave + (lane >> 2);
+  const uint32_t c_off = uint32_t(lane >> 2) * m.c_slot + (lane & 3) * (D / 8), s_off = uint32_t(lane >> 2) * m.s_slot;
   auto fetch = [&](bool isv, int t) __attribute__((always_inline)) {
     const int gq = pager.granule(4 * t + wave);
     const int e = pager.entry(gq);
     const uint8_t* cp = (isv ? m.vc : m.kc) + pager.offset(gq, e, m.c_blk, m.c_slot, ch);
     const uint8_t* sp = (isv ? m.vs : m.ks) + pager.offset(gq, e, m.s_blk, m.s_slot, sh);
-    const uint32_t in = uint32_t(min(t * TILE + srow, pager.last_key) - 16 * gq);
     Staged x;
-    x.u = load_units<D>(cp + (in * m.c_slot + (lane & 3) * (D / 8)));
-    x.s = load_scales<D>(sp + in * m.s_slot);
+    x.u = load_units<D>(cp + min(c_off, pager.limit(gq, m.c_slot) + 3 * (D / 8)));
+    x.s = load_scales<D>(sp + min(s_off, pager.limit(gq, m.s_slot)));
     return x;
   };
   auto put = [&](const Staged& x, unsigned char* tile, bool isv) __attribute__((always_inline)) {
@@ -841,6 +980,22 @@ template <int DT, int BITS, int D, bool SPLIT> int launch_rows64(const Mx4Args& 
   return 0;
 }
 
+// Whether the FAST forms serve a launch.
+template <int BITS> bool fast_of(const AttnArgs& a) {
+  return BITS != 64 && a.fxp_scale <= (BITS == 16 ? 16384.0f : 4194304.0f) && !a.alibi && a.scale_log2 > 0.0f &&
+         !(a.softcap_log2 > 0.0f);
+}
+
+template <int DT, int BITS, int D, bool SPLIT> void launch_rows16(const Mx4Args& m, dim3 grid, hipStream_t st) {
+  if constexpr (BITS != 64) {
+    if (fast_of<BITS>(m.a)) {
+      attn_mx4_rows16_kernel<DT, BITS, D, SPLIT, true><<<grid, kThreads, 0, st>>>(m);
+      return;
+    }
+  }
+  attn_mx4_rows16_kernel<DT, BITS, D, SPLIT, false><<<grid, kThreads, 0, st>>>(m);
+}
+
 template <int DT, int BITS, int D>
 int launch_mx4(Mx4Args m, const Mx4Plan& p, int num_requests, int max_query_len, int64_t num_tokens, hipStream_t st) {
   AttnArgs& a = m.a;
@@ -869,10 +1024,10 @@ int launch_mx4(Mx4Args m, const Mx4Plan& p, int num_requests, int max_query_len,
   }
   const dim3 grid(unsigned(num_requests * a.num_kv_heads), unsigned(qtiles), unsigned(p.splits));
   if (!split) {
-    attn_mx4_rows16_kernel<DT, BITS, D, false><<<grid, kThreads, 0, st>>>(m);
+    launch_rows16<DT, BITS, D, false>(m, grid, st);
     return launch_status();
   }
-  attn_mx4_rows16_kernel<DT, BITS, D, true><<<grid, kThreads, 0, st>>>(m);
+  launch_rows16<DT, BITS, D, true>(m, grid, st);
   const int64_t ws_rows = a.tok_cap > 0 ? int64_t(num_requests) * a.tok_cap : num_tokens;
   attn_mx4_combine_kernel<DT, BITS, D>
       <<<dim3(unsigned(cdiv(ws_rows * a.num_heads * (D / 2), 256))), 256, 0, st>>>(a);
