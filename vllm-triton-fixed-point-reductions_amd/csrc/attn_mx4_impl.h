@@ -613,7 +613,11 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
 // SPLIT: the chunks of a row tile are dealt evenly to pq_splits workgroups; the
 // first folds its chunks and leaves the folded state as one record, the others
 // a record per chunk.
-template <int DT, int BITS, int D, bool SPLIT>
+//
+// FAST as in the 16-row kernel, and over a softcap too (CAP): the softcap is
+// monotone, so the chunk maximum is the capped maximum of the raw scores, and
+// only phase 1 computes a score's tanh.
+template <int DT, int BITS, int D, bool SPLIT, bool FAST, bool CAP>
 __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void attn_mx4_rows64_kernel(Mx4Args m) {
   const AttnArgs& a = m.a;
   using TR = Traits<DT>;
@@ -625,8 +629,9 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
 
   const int tid = threadIdx.x, lane = tid & 63, kg = lane >> 4, i16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = blockIdx.x % a.num_kv_heads;
-  int r = blockIdx.x / a.num_kv_heads, rtile = int(gridDim.y) - 1 - int(blockIdx.y);  // the longest row tiles first
+  int r = int(quotient(blockIdx.x, m.by_heads));
+  const int g = int(blockIdx.x) - r * a.num_kv_heads;
+  int rtile = int(gridDim.y) - 1 - int(blockIdx.y);  // the longest row tiles first
   if (a.pq_blocks > 0) {
     r = __builtin_amdgcn_readfirstlane(flat_block(a, a.pq_blocks - 1 - r, rtile));
     rtile = __builtin_amdgcn_readfirstlane(rtile);
@@ -641,8 +646,8 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
   if (row0 >= rows_total || rows_total < a.pq_rows) return;  // uniform
   const int wrow0 = row0 + 16 * wave;
 
-  const int i_min = row0 / a.group;
-  const int i_max = min(rows_total - 1, row0 + PQROWS - 1) / a.group;
+  const int i_min = int(quotient(uint32_t(row0), m.by_group));
+  const int i_max = int(quotient(uint32_t(min(rows_total - 1, row0 + PQROWS - 1)), m.by_group));
   const int hi = a.causal ? min(seq_len, ctx + i_max + 1) : seq_len;
   const int lo = a.window > 0 ? max(0, ctx + i_min - a.window + 1) : 0;
   const int t_lo = lo / TILE;
@@ -659,6 +664,81 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
   const Pager pager = make_pager(a, r, seq_len);
   const uint32_t ch = uint32_t(g) * m.c_head, sh = uint32_t(g) * m.s_head;
 
+  auto live_lo = [&](int c) { return max(c * CT, t_lo); };
+  auto live_hi = [&](int c) { return min(c * CT + CT, t_hi); };
+  // The steps of chunk c: phase 0 takes K tiles ta + 2 k, ta + 2 k + 1 (the last
+  // one twice where they are odd), phase 1 K and V of tile ta + k.
+  struct Step {
+    int c, phase, k, ta, n;  // (first live tile and live tiles of c)
+  };
+  auto first_step = [&](int c) { return Step{c, 0, 0, live_lo(c), live_hi(c) - live_lo(c)}; };
+  auto next = [&](Step s) {
+    ++s.k;
+    if (s.phase == 0) {
+      if (2 * s.k >= s.n) {
+        s.phase = 1;
+        s.k = 0;
+      }
+    } else if (s.k >= s.n) {
+      if (s.c + 1 < c_hi) s = first_step(s.c + 1);
+      else s.k = s.n - 1;  // past the end: the last step again
+    }
+    return s;
+  };
+  auto tile0 = [&](const Step& s) { return s.ta + (s.phase ? s.k : 2 * s.k); };
+  auto tile1 = [&](const Step& s) { return s.ta + (s.phase ? s.k : min(2 * s.k + 1, s.n - 1)); };
+
+  // Staging: the wave moves the tile's granule `wave`, lane l row l / 4, units
+  // l % 4. The table entries of a step are loaded a step before its tiles.
+  struct Staged {
+    Units<D> u;
+    Scales<D> s;
+  };
+  const int srow = 16 * wave + (lane >> 2);
+  const uint32_t c_off = uint32_t(lane >> 2) * m.c_slot + (lane & 3) * (D / 8), s_off = uint32_t(lane >> 2) * m.s_slot;
+  auto fetch = [&](const uint8_t* codes, const uint8_t* scales, int t, int e) __attribute__((always_inline)) {
+    const int gq = pager.granule(4 * t + wave);
+    const uint8_t* cp = codes + pager.offset(gq, e, m.c_blk, m.c_slot, ch);
+    const uint8_t* sp = scales + pager.offset(gq, e, m.s_blk, m.s_slot, sh);
+    Staged x;
+    x.u = load_units<D>(cp + min(c_off, pager.limit(gq, m.c_slot) + 3 * (D / 8)));
+    x.s = load_scales<D>(sp + min(s_off, pager.limit(gq, m.s_slot)));
+    return x;
+  };
+  unsigned kwr[QS], vwr[QS];
+#pragma unroll
+  for (int j = 0; j < QS; ++j) {
+    kwr[j] = srow * L::ROWB + (((4 * j + (lane & 3)) ^ L::kswz(srow)) << 4);
+    vwr[j] = srow * L::ROWB + (((4 * j + (lane & 3)) ^ L::vswz(srow)) << 4);
+  }
+  auto put = [&](const Staged& x, unsigned char* tile, const unsigned (&at)[QS]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < QS; ++j)
+      lds_store16(tile + at[j], mx4::unpack8<DT>(x.u.w[j], mx4::scale_of<DT>(x.s.w[j / 4], j % 4)));
+  };
+  auto tile_at = [&](int b, int j) { return lds + (2 * b + j) * L::TILEB; };
+  Staged r0, r1;
+  int e0 = 0, e1 = 0;
+  auto entries = [&](const Step& s) __attribute__((always_inline)) {
+    e0 = pager.entry(pager.granule(4 * tile0(s) + wave));
+    e1 = pager.entry(pager.granule(4 * tile1(s) + wave));
+  };
+  auto fetch_step = [&](const Step& s) __attribute__((always_inline)) {
+    r0 = fetch(m.kc, m.ks, tile0(s), e0);
+    r1 = fetch(s.phase ? m.vc : m.kc, s.phase ? m.vs : m.ks, tile1(s), e1);
+  };
+  auto put_step = [&](const Step& s, int b) __attribute__((always_inline)) {
+    put(r0, tile_at(b, 0), kwr);
+    if (s.phase) put(r1, tile_at(b, 1), vwr);  // uniform
+    else put(r1, tile_at(b, 1), kwr);
+  };
+  Step ahead{};  // the step whose tiles are in registers
+  if (c_lo < c_hi) {
+    ahead = first_step(c_lo);
+    entries(ahead);
+    fetch_step(ahead);
+  }
+
   // The lane's query row.
   const RowInfo me = row_at(m, g, q_start, q_len, ctx, seq_len, wrow0 + i16);
   u32x4 qf[QS];
@@ -671,33 +751,9 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
   const int ks = me.valid ? me.kstart : 0x7fffffff;
   const int ke = me.valid ? me.kend : 0;
   const int qp = me.qpos;
-  const float slope = a.alibi ? a.alibi[me.head] : 0.0f;
-
-  // Staging: the wave moves the tile's granule `wave`, lane l row l / 4, units
-  // l % 4.
-  struct Staged {
-    Units<D> u;
-    Scales<D> s;
-  };
-  const int srow = 16 * wave + (lane >> 2);
-  const uint32_t c_off = uint32_t(lane >> 2) * m.c_slot + (lane & 3) * (D / 8), s_off = uint32_t(lane >> 2) * m.s_slot;
-  auto fetch = [&](bool isv, int t) __attribute__((always_inline)) {
-    const int gq = pager.granule(4 * t + wave);
-    const int e = pager.entry(gq);
-    const uint8_t* cp = (isv ? m.vc : m.kc) + pager.offset(gq, e, m.c_blk, m.c_slot, ch);
-    const uint8_t* sp = (isv ? m.vs : m.ks) + pager.offset(gq, e, m.s_blk, m.s_slot, sh);
-    Staged x;
-    x.u = load_units<D>(cp + min(c_off, pager.limit(gq, m.c_slot) + 3 * (D / 8)));
-    x.s = load_scales<D>(sp + min(s_off, pager.limit(gq, m.s_slot)));
-    return x;
-  };
-  auto put = [&](const Staged& x, unsigned char* tile, bool isv) __attribute__((always_inline)) {
-    unsigned char* row = tile + srow * L::ROWB;
-    const int sw = isv ? L::vswz(srow) : L::kswz(srow);
-#pragma unroll
-    for (int j = 0; j < QS; ++j)
-      lds_store16(row + (((4 * j + (lane & 3)) ^ sw) << 4),
-                  mx4::unpack8<DT>(x.u.w[j], mx4::scale_of<DT>(x.s.w[j / 4], j % 4)));
+  const float slope = !FAST && a.alibi ? a.alibi[me.head] : 0.0f;
+  auto tile_whole = [&](int t) -> bool {
+    return __builtin_amdgcn_ballot_w64(!(ks <= t * TILE && t * TILE + TILE <= ke)) == 0;
   };
 
   // LDS offsets of the score MFMAs' K rows pi(i16) (step s: + 32 rows, which
@@ -738,95 +794,103 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
     for (int b = 0; b < DBLK; ++b) wp[4 * b] = acc4{w[b][0], w[b][1], w[b][2], w[b][3]};
   };
 
-  auto live_lo = [&](int c) { return max(c * CT, t_lo); };
-  auto live_hi = [&](int c) { return min(c * CT + CT, t_hi); };
-  // The steps of chunk c: phase 0 takes K tiles ta + 2 k, ta + 2 k + 1 (the last
-  // one twice where they are odd), phase 1 K and V of tile ta + k.
-  struct Step {
-    int c, phase, k;
-  };
-  auto next = [&](Step s) {
-    const int n = live_hi(s.c) - live_lo(s.c);
-    ++s.k;
-    if (s.phase == 0 && 2 * s.k >= n) {
-      s.phase = 1;
-      s.k = 0;
-    } else if (s.phase == 1 && s.k >= n) {
-      if (s.c + 1 < c_hi) {
-        ++s.c;
-        s.phase = 0;
-        s.k = 0;
-      } else {
-        s.k = n - 1;  // past the end: the last step again
-      }
-    }
-    return s;
-  };
-  Staged r0, r1;
-  auto fetch_step = [&](const Step& s) __attribute__((always_inline)) {
-    const int ta = live_lo(s.c), te = live_hi(s.c);
-    const bool kv = s.phase == 1;
-    r0 = fetch(false, ta + (kv ? s.k : 2 * s.k));
-    r1 = fetch(kv, kv ? ta + s.k : min(ta + 2 * s.k + 1, te - 1));
-  };
   int buf = 0;
-  auto tile_at = [&](int b, int j) { return lds + (2 * b + j) * L::TILEB; };
-
+  // The four score MFMA chains of a K tile; a chain's LDS reads go out before
+  // the chain before it is waited for.
   auto scores_of = [&](const unsigned char* tile, auto&& fn) __attribute__((always_inline)) {
+    u32x4 kf[2][QS];
+    auto issue = [&](auto qc) __attribute__((always_inline)) {
+      constexpr int q = decltype(qc)::value;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+      for (int j = 0; j < QS; ++j) kf[q & 1][j] = lds_load16(tile + (q >> 1) * 32 * L::ROWB + koff[q & 1][j]);
+    };
+    issue(std::integral_constant<int, 0>{});
+    f32x4 accs[2];
+    static_for<4>([&](auto qc) __attribute__((always_inline)) {
+      constexpr int q = decltype(qc)::value;
+      if constexpr (q + 1 < 4) issue(std::integral_constant<int, q + 1>{});
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < QS; ++j)
-        acc = TR::mma(lds_load16(tile + (q >> 1) * 32 * L::ROWB + koff[q & 1][j]), qf[j], acc);
-      fn(q, acc);
-    }
+      for (int j = 0; j < QS; ++j) acc = TR::mma(kf[q & 1][j], qf[j], acc);
+      accs[q & 1] = acc;
+      if constexpr (q > 0) fn(std::integral_constant<int, q - 1>{}, accs[(q - 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    fn(std::integral_constant<int, 3>{}, accs[1]);
   };
-  auto masked = [&](const f32x4& acc, int t, int q, float (&sc)[4]) __attribute__((always_inline)) {
+  auto capped = [&](float x) { return softcapped(x, a.softcap_log2); };
+  // Scores of chain q for the lane's row and keys t * TILE + 32 (q / 2) + 8 kg +
+  // 4 (q % 2) + e. (RAW: before the softcap; the mask is -inf, a score is not.)
+  auto chain_scores = [&](const f32x4& acc, int t, int q, bool whole, auto raw_tag, float (&sc)[4])
+                          __attribute__((always_inline)) {
+    constexpr bool RAW = decltype(raw_tag)::value;
     const int key0 = t * TILE + 32 * (q >> 1) + 8 * kg + 4 * (q & 1);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float x = __fmul_rn(acc[e], a.scale_log2);
-      if (a.softcap_log2 > 0.0f) x = softcapped(x, a.softcap_log2);
-      if (a.alibi) x = x + slope * static_cast<float>(key0 + e - qp);
-      sc[e] = (key0 + e >= ks && key0 + e < ke) ? x : -__builtin_inff();
+      if constexpr (!FAST) {
+        if (a.softcap_log2 > 0.0f) x = capped(x);
+        if (a.alibi) x = x + slope * static_cast<float>(key0 + e - qp);
+      } else if constexpr (CAP) {
+        x = RAW ? fmaxf(x, -kFltMax) : capped(x);
+      }
+      sc[e] = (whole || (key0 + e >= ks && key0 + e < ke)) ? x : -__builtin_inff();
     }
   };
+  [[maybe_unused]] const float vlim = (BITS == 16 ? 32767.0f : 4194304.0f) / a.fxp_scale;
 
   if (c_lo < c_hi) {
-    Step cur{c_lo, 0, 0}, ahead = next(cur);
-    fetch_step(cur);
-    put(r0, tile_at(0, 0), false);
-    put(r1, tile_at(0, 1), false);
+    put_step(ahead, 0);
+    Step after = next(ahead);
+    entries(after);
+    ahead = after;
     fetch_step(ahead);
+    after = next(ahead);
+    entries(after);
     // One step: publish its tiles, unpack the next step's, load the one after.
     auto step_begin = [&]() __attribute__((always_inline)) {
       lds_barrier();
-      put(r0, tile_at(buf ^ 1, 0), false);
-      put(r1, tile_at(buf ^ 1, 1), ahead.phase == 1);
-      cur = ahead;
-      ahead = next(ahead);
+      put_step(ahead, buf ^ 1);
+      ahead = after;
       fetch_step(ahead);
+      after = next(ahead);
+      entries(after);
     };
     for (int c = c_lo; c < c_hi; ++c) {
       const int ta = live_lo(c), te = live_hi(c);
-      float mx = -__builtin_inff();
+      float mx = -__builtin_inff(), mraw = -__builtin_inff();
+      // phase 0: the chunk's row maxima
       for (int t = ta; t < te; t += 2) {
         step_begin();
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          if (t + j < te)
-            scores_of(tile_at(buf, j), [&](int q, const f32x4& acc) __attribute__((always_inline)) {
+          if (t + j >= te) continue;  // uniform
+          if (FAST && tile_whole(t + j)) {
+            scores_of(tile_at(buf, j), [&](auto, const f32x4& acc) __attribute__((always_inline)) {
+              mraw = fmaxf(fmaxf(mraw, fmaxf(acc[0], acc[1])), fmaxf(acc[2], acc[3]));
+            });
+            if constexpr (CAP) mraw = fmaxf(mraw, -kFltMax);  // keys were seen
+          } else {
+            scores_of(tile_at(buf, j), [&](auto qc, const f32x4& acc) __attribute__((always_inline)) {
               float sc[4];
-              masked(acc, t + j, q, sc);
+              chain_scores(acc, t + j, decltype(qc)::value, false, std::true_type{}, sc);
               mx = fmaxf(fmaxf(mx, fmaxf(sc[0], sc[1])), fmaxf(sc[2], sc[3]));
             });
+          }
         }
         buf ^= 1;
       }
+      if constexpr (FAST) {
+        float m1 = __fmul_rn(mraw, a.scale_log2);
+        if constexpr (CAP) m1 = mraw != -__builtin_inff() ? fmaxf(m1, -kFltMax) : m1;
+        mx = fmaxf(mx, m1);
+      }
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      if constexpr (CAP) mx = mx != -__builtin_inff() ? capped(mx) : mx;
       const float mrow = mx != -__builtin_inff() ? mx : 0.0f;  // no key: pin to 0
+      // phase 1: weights and weighted V. FAST: the sums carry kRound per added
+      // term, taken out at the chunk's end.
       AccT den = 0;
       AccT wv[DBLK][4];
 #pragma unroll
@@ -836,46 +900,127 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
       for (int t = ta; t < te; ++t) {
         step_begin();
         u32x4 pb[2];
-        scores_of(tile_at(buf, 0), [&](int q, const f32x4& acc) __attribute__((always_inline)) {
-          float sc[4];
-          masked(acc, t, q, sc);
-          uint32_t p16[4];
+        auto weights = [&](auto whole_tag) __attribute__((always_inline)) {
+          constexpr bool WHOLE = decltype(whole_tag)::value;
+          scores_of(tile_at(buf, 0), [&](auto qc, const f32x4& acc) __attribute__((always_inline)) {
+            constexpr int q = decltype(qc)::value, s = q >> 1, h = q & 1;
+            float sc[4], w[4];
+            chain_scores(acc, t, q, WHOLE, std::false_type{}, sc);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float w = __builtin_amdgcn_exp2f(sc[e] - mrow);
-            den = wadd<BITS>(den, quant<BITS>(__fmul_rn(w, a.fxp_scale)));
-            p16[e] = Io<DT>::store(w);
-          }
-          pb[q >> 1][2 * (q & 1)] = p16[0] | (p16[1] << 16);
-          pb[q >> 1][2 * (q & 1) + 1] = p16[2] | (p16[3] << 16);
-        });
+            for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(sc[e] - mrow);
+            if constexpr (FAST) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)  // (the maximum: NaN counts as 0)
+                den = AccT(uint32_t(den) + __float_as_uint(fmaxf(__builtin_fmaf(w[e], a.fxp_scale, kRoundF), kRoundF)));
+              pb[s][2 * h] = p_pack2<DT>(w[0], w[1]);
+              pb[s][2 * h + 1] = p_pack2<DT>(w[2], w[3]);
+            } else {
+              uint32_t p16[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                den = wadd<BITS>(den, quant<BITS>(__fmul_rn(w[e], a.fxp_scale)));
+                p16[e] = Io<DT>::store(w[e]);
+              }
+              pb[s][2 * h] = p16[0] | (p16[1] << 16);
+              pb[s][2 * h + 1] = p16[2] | (p16[3] << 16);
+            }
+          });
+        };
+        if (FAST && tile_whole(t)) weights(std::true_type{});
+        else weights(std::false_type{});
+
+        // d blocks, the next one's V reads before this one's MFMAs
         const unsigned char* vt = tile_at(buf, 1);
+        u32x2 vr[2][2][2];
+        auto issue_v = [&](auto bc) __attribute__((always_inline)) {
+          constexpr int b = decltype(bc)::value;
 #pragma unroll
-        for (int b = 0; b < DBLK; ++b) {
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) vr[b & 1][s][h] = lds_load_tr8(vt + s * 32 * L::ROWB + (vrd[h] ^ (b << 5)));
+        };
+        issue_v(std::integral_constant<int, 0>{});
+        f32x4 accv[FAST ? DBLK : 1];
+        float vmax = 0.0f;
+        static_for<DBLK>([&](auto bc) __attribute__((always_inline)) {
+          constexpr int b = decltype(bc)::value;
+          if constexpr (b + 1 < DBLK) issue_v(std::integral_constant<int, b + 1>{});
           f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const u32x2 lo2 = lds_load_tr8(vt + s * 32 * L::ROWB + (vrd[0] ^ (b << 5)));
-            const u32x2 hi2 = lds_load_tr8(vt + s * 32 * L::ROWB + (vrd[1] ^ (b << 5)));
-            acc = TR::mma(u32x4{lo2[0], lo2[1], hi2[0], hi2[1]}, pb[s], acc);
-          }
+          for (int s = 0; s < 2; ++s)
+            acc = TR::mma(u32x4{vr[b & 1][s][0][0], vr[b & 1][s][0][1], vr[b & 1][s][1][0], vr[b & 1][s][1][1]}, pb[s], acc);
+          if constexpr (FAST) {
+            // block b - 1's terms while block b's MFMAs run
+            accv[b] = acc;
+            if constexpr (b > 0) vmax = absmax4(vmax, accv[b - 1]);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) wv[b][e] = wadd<BITS>(wv[b][e], quant<BITS>(__fmul_rn(acc[e], a.fxp_scale)));
+            for (int e = 0; e < 4; ++e) wv[b][e] = wadd<BITS>(wv[b][e], quant<BITS>(__fmul_rn(acc[e], a.fxp_scale)));
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (FAST) {
+          vmax = absmax4(vmax, accv[DBLK - 1]);
+          auto term = [&](float x) { return __float_as_uint(__builtin_fmaf(x, a.fxp_scale, kRoundF)); };
+#pragma unroll
+          for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) wv[b][e] = AccT(uint32_t(wv[b][e]) + term(accv[b][e]));
+          if (__builtin_amdgcn_ballot_w64(!(vmax < vlim)) != 0) {  // uniform: out of the constant's range
+#pragma unroll
+            for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const AccT without = AccT(uint32_t(wv[b][e]) - term(accv[b][e]));
+                wv[b][e] = AccT(uint32_t(wadd<BITS>(without, quant<BITS>(__fmul_rn(accv[b][e], a.fxp_scale)))) + kRound);
+              }
+          }
         }
         buf ^= 1;
+      }
+      if constexpr (FAST) {
+        const uint32_t terms = uint32_t(te - ta) * kRound;
+        den = AccT(uint32_t(den) - 16u * terms);
+#pragma unroll
+        for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) wv[b][e] = AccT(uint32_t(wv[b][e]) - terms);
       }
       den = wadd<BITS>(den, __shfl_xor(den, 16, 64));
       den = wadd<BITS>(den, __shfl_xor(den, 32, 64));
       if (SPLIT && split > 0) {  // uniform
         store_record(c, mx, den, wv);
-      } else if (mx != -__builtin_inff()) {
-        float Mn, fa, fb;
-        merge_factors(Mr, mx, Mn, fa, fb);
-        Dr = wadd<BITS>(rescale<BITS>(Dr, fa), rescale<BITS>(den, fb));
+      } else if (__builtin_amdgcn_ballot_w64(Mr != -__builtin_inff()) == 0) {
+        // nothing folded yet in the wave: the chunk's own sums
 #pragma unroll
         for (int b = 0; b < DBLK; ++b)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) Wr[b][e] = wadd<BITS>(rescale<BITS>(Wr[b][e], fa), rescale<BITS>(wv[b][e], fb));
+          for (int e = 0; e < 4; ++e) Wr[b][e] = wv[b][e];
+        Dr = den;
+        Mr = mx;
+      } else if (mx != -__builtin_inff()) {
+        float Mn, fa, fb;
+        merge_factors(Mr, mx, Mn, fa, fb);
+        // fa or fb is 1 (unless both maxima are +inf), and rescale(x, 1) = x for
+        // 16- and 32-bit sums: one side is rescaled
+        const bool one_a = fa == 1.0f;
+        if (BITS != 64 && __builtin_amdgcn_ballot_w64(!(one_a || fb == 1.0f)) == 0) {
+          const float f = one_a ? fb : fa;
+          Dr = wadd<BITS>(rescale<BITS>(one_a ? den : Dr, f), one_a ? Dr : den);
+#pragma unroll
+          for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const AccT x = one_a ? wv[b][e] : Wr[b][e], y = one_a ? Wr[b][e] : wv[b][e];
+              Wr[b][e] = wadd<BITS>(rescale<BITS>(x, f), y);
+            }
+        } else {
+          Dr = wadd<BITS>(rescale<BITS>(Dr, fa), rescale<BITS>(den, fb));
+#pragma unroll
+          for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) Wr[b][e] = wadd<BITS>(rescale<BITS>(Wr[b][e], fa), rescale<BITS>(wv[b][e], fb));
+        }
         Mr = Mn;
       }
     }
@@ -891,13 +1036,18 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
       }
     }
   } else if (me.valid) {
+    // the row's quotients over one denominator by its rounded reciprocal: the
+    // bits of div_rn
     const float den_f = fmaxf(acc_f32<BITS>(Dr, a.fxp_inv), 1.0e-6f);
+    const float rcp = div_rn(1.0f, den_f);
     T* orow = static_cast<T*>(a.o) + me.token * a.so_t + int64_t(me.head) * a.so_h;
 #pragma unroll
     for (int b = 0; b < DBLK; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        orow[b * 16 + 4 * kg + e] = Io<DT>::store(div_rn(acc_f32<BITS>(Wr[b][e], a.fxp_inv), den_f));
+      for (int e = 0; e < 4; ++e) {
+        const float num = acc_f32<BITS>(Wr[b][e], a.fxp_inv);
+        orow[b * 16 + 4 * kg + e] = Io<DT>::store(BITS == 64 ? div_rn(num, den_f) : div_rn_by_recip(num, den_f, rcp));
+      }
   }
 }
 
@@ -966,8 +1116,14 @@ __global__ __launch_bounds__(256) void attn_mx4_combine_kernel(AttnArgs a) {
 // ---------------------------------------------------------------------------
 // Launches.
 
-template <int DT, int BITS, int D, bool SPLIT> int launch_rows64(const Mx4Args& m, dim3 grid, hipStream_t st) {
-  auto kern = attn_mx4_rows64_kernel<DT, BITS, D, SPLIT>;
+// Whether the FAST forms serve a launch (the 16-row one without a softcap).
+template <int BITS> bool fast_of(const AttnArgs& a) {
+  return BITS != 64 && a.fxp_scale <= (BITS == 16 ? 16384.0f : 4194304.0f) && !a.alibi && a.scale_log2 > 0.0f;
+}
+
+template <int DT, int BITS, int D, bool SPLIT, bool FAST, bool CAP>
+int launch_rows64(const Mx4Args& m, dim3 grid, hipStream_t st) {
+  auto kern = attn_mx4_rows64_kernel<DT, BITS, D, SPLIT, FAST, CAP>;
   constexpr int lds = 4 * Lds<D>::TILEB;
   static bool attr_done = false;  // benign race: the attribute is idempotent
   if (!attr_done) {
@@ -980,15 +1136,18 @@ template <int DT, int BITS, int D, bool SPLIT> int launch_rows64(const Mx4Args& 
   return 0;
 }
 
-// Whether the FAST forms serve a launch.
-template <int BITS> bool fast_of(const AttnArgs& a) {
-  return BITS != 64 && a.fxp_scale <= (BITS == 16 ? 16384.0f : 4194304.0f) && !a.alibi && a.scale_log2 > 0.0f &&
-         !(a.softcap_log2 > 0.0f);
+template <int DT, int BITS, int D, bool SPLIT> int launch_rows64(const Mx4Args& m, dim3 grid, hipStream_t st) {
+  if constexpr (BITS != 64) {
+    if (fast_of<BITS>(m.a))
+      return m.a.softcap_log2 > 0.0f ? launch_rows64<DT, BITS, D, SPLIT, true, true>(m, grid, st)
+                                     : launch_rows64<DT, BITS, D, SPLIT, true, false>(m, grid, st);
+  }
+  return launch_rows64<DT, BITS, D, SPLIT, false, false>(m, grid, st);
 }
 
 template <int DT, int BITS, int D, bool SPLIT> void launch_rows16(const Mx4Args& m, dim3 grid, hipStream_t st) {
   if constexpr (BITS != 64) {
-    if (fast_of<BITS>(m.a)) {
+    if (fast_of<BITS>(m.a) && !(m.a.softcap_log2 > 0.0f)) {
       attn_mx4_rows16_kernel<DT, BITS, D, SPLIT, true><<<grid, kThreads, 0, st>>>(m);
       return;
     }
