@@ -1051,67 +1051,171 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
   }
 }
 
-// Folds the records of each (token, head) in ascending chunk order and divides:
-// a thread takes two consecutive d of a row.
-template <int DT, int BITS, int D>
+// Folds the records of each (token, head) in ascending chunk order and divides.
+// The fold's factors do not depend on the sums, so 64 chunks' maxima are scanned
+// at once, a lane each; a chunk that raises the running maximum (a few of a
+// row's) rescales the sums, the terms of the others are only added, in any
+// order. A row's records are loaded a batch ahead of their use.
+//
+// A wave takes a row, D / 64 elements a lane, or (WIDE, for launches of few rows
+// of many chunks) the four waves of a workgroup take 64 elements of a row: wave 0
+// the chunks of a block of 64 up to the last one that raises the maximum, then
+// each a quarter of the rest. One request over 131072 keys, 32 rows of 256
+// records: 43 us with a thread folding step by step, 21.6 with a wave a row, 9
+// with four (WIDE).
+template <int DT, int BITS, int D, bool WIDE>
 __global__ __launch_bounds__(256) void attn_mx4_combine_kernel(AttnArgs a) {
   using T = typename Traits<DT>::T;
   using AccT = typename AccOf<BITS>::T;
-  constexpr int V = 2, PER = D / V;
+  constexpr int V = WIDE ? 1 : D / 64, PARTS = WIDE ? D / 64 : 1;
   typedef AccT accv __attribute__((ext_vector_type(V)));
-  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
-  const uint32_t th = idx / PER;
-  const int d = int(idx % PER) * V;
-  const uint32_t wrow = th / uint32_t(a.num_heads);
+  __shared__ AccT part_w[WIDE ? 4 : 1][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = WIDE ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const uint32_t unit =
+      WIDE ? blockIdx.x : uint32_t(__builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6)));
+  const uint32_t th = unit / PARTS;
+  const int d = int(unit % PARTS) * 64 + lane * V;
+  const uint32_t wrow = th / uint32_t(a.num_heads);  // (past the last row: past every request)
   const int head = int(th - wrow * uint32_t(a.num_heads));
   int64_t token = wrow;
   if (a.tok_cap > 0) {
     const uint32_t r = wrow / uint32_t(a.tok_cap);
     if (r >= uint32_t(a.num_requests)) return;
-    const int i = int(wrow - r * uint32_t(a.tok_cap)), q0 = a.qsl[r], q_len = a.qsl[r + 1] - q0;
+    const int i = int(wrow - r * uint32_t(a.tok_cap)), q0 = ((ConstI32)a.qsl)[r], q_len = ((ConstI32)a.qsl)[r + 1] - q0;
     if (i >= q_len || (a.pq_rows > 0 && q_len * a.group >= a.pq_rows)) return;
     token = q0 + i;
     if (token < 0 || token >= a.num_tokens) return;
   } else {
     // tokens outside query_start_loc's range belong to no request and are left
     // as they are
-    const int64_t used = min<int64_t>(a.num_tokens, a.qsl[a.num_requests]);
-    if (token < a.qsl[0] || token >= used) return;
+    const int64_t used = min<int64_t>(a.num_tokens, ((ConstI32)a.qsl)[a.num_requests]);
+    if (token < ((ConstI32)a.qsl)[0] || token >= used) return;
   }
-  const int c0 = max(0, a.crange[2 * int64_t(th)]), c1 = min(a.chunk_slots, a.crange[2 * int64_t(th) + 1]);
+  const float* pm_p = a.pmax + int64_t(th) * a.chunk_slots;
   const AccT* den_p = static_cast<const AccT*>(a.den_ws) + int64_t(th) * a.chunk_slots;
   const AccT* wv_p = static_cast<const AccT*>(a.wv_ws) + int64_t(th) * a.chunk_slots * D + d;
-  const float* pm_p = a.pmax + int64_t(th) * a.chunk_slots;
+  const int c0 = max(0, __builtin_amdgcn_readfirstlane(a.crange[2 * int64_t(th)]));
+  const int c1 = min(a.chunk_slots, __builtin_amdgcn_readfirstlane(a.crange[2 * int64_t(th) + 1]));
   float M = -__builtin_inff();
-  AccT Dn = 0, W[V] = {0, 0};
-  constexpr int NB = 8;
-  for (int cb = c0; cb < c1; cb += NB) {
-    float mc[NB];
-    AccT dc[NB];
-    accv wc[NB];
+  AccT Dn = 0, W[V];  // (Dn: wave 0's)
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      const int c = min(cb + k, c1 - 1);
-      mc[k] = pm_p[c];
-      dc[k] = den_p[c];
-      wc[k] = *reinterpret_cast<const accv*>(wv_p + int64_t(c) * D);
+  for (int v = 0; v < V; ++v) W[v] = 0;
+  constexpr int NB = 16, NH = 64 / NB;
+  accv wc[2][NB];
+  auto load = [&](int cb, accv (&w)[NB]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < NB; ++k) w[k] = *reinterpret_cast<const accv*>(wv_p + int64_t(min(cb + k, c1 - 1)) * D);
+  };
+  // the waves' sums of added terms into wave 0's
+  auto gather = [&]() __attribute__((always_inline)) {
+    if constexpr (WIDE) {
+      part_w[wave][lane] = W[0];
+      __syncthreads();
+      if (wave == 0) {
+        W[0] = wadd<BITS>(wadd<BITS>(part_w[0][lane], part_w[1][lane]), wadd<BITS>(part_w[2][lane], part_w[3][lane]));
+      } else {
+        W[0] = 0;
+      }
+      __syncthreads();
     }
+  };
+  for (int cs = c0; cs < c1; cs += 64) {
+    if constexpr (WIDE) load(cs + wave * NB, wc[0]);
+    else load(cs, wc[0]);
+    // this lane's chunk: its maximum, and the factors of its fold
+    const int cl = min(cs + lane, c1 - 1);
+    const float mc = cs + lane < c1 ? pm_p[cl] : -__builtin_inff();
+    const AccT dc = den_p[cl];
+    float incl = mc;
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      if (cb + k >= c1 || mc[k] == -__builtin_inff()) continue;
-      float Mn, fa, fb;
-      merge_factors(M, mc[k], Mn, fa, fb);
-      Dn = wadd<BITS>(rescale<BITS>(Dn, fa), rescale<BITS>(dc[k], fb));
+    for (int o = 1; o < 64; o <<= 1) {
+      const float x = __shfl_up(incl, o, 64);
+      if (lane >= o) incl = fmaxf(incl, x);
+    }
+    float before = __shfl_up(incl, 1, 64);
+    before = lane == 0 ? M : fmaxf(M, before);
+    float Mn, fa, fb;
+    merge_factors(before, mc, Mn, fa, fb);
+    const AccT dr = rescale<BITS>(dc, fb);
+    const uint64_t seen = __builtin_amdgcn_ballot_w64(mc != -__builtin_inff());
+    // (rescale(x, 1) = x for 16- and 32-bit sums)
+    const uint64_t moves = BITS == 64 ? seen : seen & __builtin_amdgcn_ballot_w64(fa != 1.0f);
+    M = __shfl(fmaxf(before, incl), 63, 64);
+    auto term = [&](int l, const accv& w) __attribute__((always_inline)) {
+      const float f = __uint_as_float(uint32_t(__builtin_amdgcn_readlane(int(__float_as_uint(fb)), l)));
 #pragma unroll
-      for (int v = 0; v < V; ++v) W[v] = wadd<BITS>(rescale<BITS>(W[v], fa), rescale<BITS>(wc[k][v], fb));
-      M = Mn;
+      for (int v = 0; v < V; ++v) W[v] = wadd<BITS>(W[v], rescale<BITS>(w[v], f));
+    };
+    auto den_term = [&](int l) -> AccT {
+      if constexpr (BITS == 64) {
+        const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(dr)), l));
+        const uint32_t hi = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(uint64_t(dr) >> 32)), l));
+        return AccT((uint64_t(hi) << 32) | lo);
+      } else {
+        return AccT(__builtin_amdgcn_readlane(int(dr), l));
+      }
+    };
+    // chunks k0 .. of the block in order, up to chunk `last`
+    auto fold = [&](int k0, int last, const accv (&w)[NB]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const int l = k0 + k;  // uniform
+        if (l > last || !((seen >> l) & 1)) continue;
+        if ((moves >> l) & 1) {
+          const float g = __uint_as_float(uint32_t(__builtin_amdgcn_readlane(int(__float_as_uint(fa)), l)));
+#pragma unroll
+          for (int v = 0; v < V; ++v) W[v] = rescale<BITS>(W[v], g);
+          Dn = rescale<BITS>(Dn, g);
+        }
+        term(l, w[k]);
+        Dn = wadd<BITS>(Dn, den_term(l));
+      }
+    };
+    if constexpr (WIDE) {
+      const int last = moves ? 63 - __builtin_clzll(moves) : -1;  // uniform, and the same in every wave
+      if (last >= 0) {
+        gather();
+        if (wave == 0) {
+          for (int h = 0; h * NB <= last; ++h) {
+            load(cs + h * NB, wc[1]);
+            fold(h * NB, last, wc[1]);
+          }
+        }
+      }
+      // the rest of the block: a quarter each
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const int l = wave * NB + k;
+        if (l > last && ((seen >> l) & 1)) term(l, wc[0][k]);
+      }
+      if (wave == 0) {
+        AccT t = lane > last && ((seen >> lane) & 1) ? dr : AccT(0);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) t = wadd<BITS>(t, __shfl_xor(t, o, 64));
+        Dn = wadd<BITS>(Dn, t);
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        if (cs + h * NB >= c1) break;  // uniform
+        if (h + 1 < NH && cs + (h + 1) * NB < c1) load(cs + (h + 1) * NB, wc[(h + 1) & 1]);
+        fold(h * NB, 63, wc[h & 1]);
+      }
     }
   }
+  gather();
+  if (wave != 0) return;
   const float den_f = fmaxf(acc_f32<BITS>(Dn, a.fxp_inv), 1.0e-6f);
   T* o = static_cast<T*>(a.o) + token * a.so_t + int64_t(head) * a.so_h + d;
 #pragma unroll
   for (int v = 0; v < V; ++v) o[v] = Io<DT>::store(div_rn(acc_f32<BITS>(W[v], a.fxp_inv), den_f));
 }
+
+// Waves of a combine launch from which each takes a row, and chunks per row up
+// to which one does: below and above, four waves share 64 elements (WIDE).
+constexpr int64_t kWideRows = 2048;
+constexpr int kWideChunks = 32;
 
 // ---------------------------------------------------------------------------
 // Launches.
@@ -1188,8 +1292,11 @@ int launch_mx4(Mx4Args m, const Mx4Plan& p, int num_requests, int max_query_len,
   }
   launch_rows16<DT, BITS, D, true>(m, grid, st);
   const int64_t ws_rows = a.tok_cap > 0 ? int64_t(num_requests) * a.tok_cap : num_tokens;
-  attn_mx4_combine_kernel<DT, BITS, D>
-      <<<dim3(unsigned(cdiv(ws_rows * a.num_heads * (D / 2), 256))), 256, 0, st>>>(a);
+  const int64_t rows = ws_rows * a.num_heads;
+  if (rows < kWideRows && a.chunk_slots > kWideChunks)
+    attn_mx4_combine_kernel<DT, BITS, D, true><<<dim3(unsigned(rows * (D / 64))), 256, 0, st>>>(a);
+  else
+    attn_mx4_combine_kernel<DT, BITS, D, false><<<dim3(unsigned(cdiv(rows, 4))), 256, 0, st>>>(a);
   return launch_status();
 }
 
