@@ -158,6 +158,7 @@ extern "C" int fxpr_unified_attention_mx4(
   m.s_head = uint32_t(stride_scales_head);
   m.by_group = reciprocal(uint32_t(num_heads / num_kv_heads));
   m.by_heads = reciprocal(uint32_t(num_kv_heads));
+  m.by_reqs = reciprocal(uint32_t(num_requests));
   a.q = q;
   a.o = o;
   a.qsl = query_start_loc;

@@ -36,7 +36,7 @@ struct Mx4Args {
   const uint8_t* ks;
   const uint8_t* vs;
   uint32_t c_blk, c_slot, c_head, s_blk, s_slot, s_head;  // bytes
-  uint32_t by_group, by_heads;  // ceil(2^32 / x): x / group and x / num_kv_heads by a high product (see quotient)
+  uint32_t by_group, by_heads, by_reqs;  // ceil(2^32 / x) of the group, kv heads and requests (see quotient)
 };
 
 // x / d with m = ceil(2^32 / d): exact while x d < 2^32 (the excess of m over
@@ -64,6 +64,19 @@ __device__ __forceinline__ RowInfo row_at(const Mx4Args& m, int g, int q_start, 
   ri.kend = a.causal ? min(seq_len, ri.qpos + 1) : seq_len;
   ri.kstart = a.window > 0 ? max(0, ri.qpos - a.window + 1) : 0;
   return ri;
+}
+
+// The request of a workgroup whose place in the launch order is request slot x
+// of a pass (a row tile, a key split) over the requests: slot x + pass, around.
+// Workgroups go to the XCDs and to the shader engines of an XCD in turn,
+// whatever those still hold, so in a grid of requests x passes one request's
+// workgroups would all go to the same engines and the longest request's engines
+// end last (prompts of 2048, 1547, 1083 and 1534 tokens, 8 kv heads: each
+// request on one engine of every XCD). Every second pass: the passes of two
+// requests then reach all four engines too.
+__device__ __forceinline__ int turned(const Mx4Args& m, int x, int pass) {
+  const uint32_t v = uint32_t(x + (pass >> 1));
+  return int(v - quotient(v, m.by_reqs) * uint32_t(m.a.num_requests));
 }
 
 // The rounding constant of the fast quantisation: for |x| 2^f < 2^22,
@@ -220,8 +233,9 @@ __device__ __forceinline__ void rows16_body(const Mx4Args& m) {
   const int tid = threadIdx.x, lane = tid & 63, kg = lane >> 4, i16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   unsigned char* stage = stage_all + wave * WAVEB;
-  const int r = int(quotient(blockIdx.x, m.by_heads)), g = int(blockIdx.x) - r * a.num_kv_heads;
+  const int slot_x = int(quotient(blockIdx.x, m.by_heads)), g = int(blockIdx.x) - slot_x * a.num_kv_heads;
   const int split = blockIdx.z;
+  const int r = turned(m, slot_x, int(blockIdx.z * gridDim.y + blockIdx.y));
   const int q_start = ((ConstI32)a.qsl)[r];
   const int q_len = ((ConstI32)a.qsl)[r + 1] - q_start;
   const int seq_len = ((ConstI32)a.seq_lens)[r];
@@ -605,10 +619,15 @@ __global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn
 // ---------------------------------------------------------------------------
 // 64 query rows, 16 a wave. A chunk's K tiles are read twice, for the row
 // maxima (two tiles a step) and, with the V tiles, for the weights, as in
-// attn_impl.h's prefill kernels. A step has two tiles in LDS (K K or K V) and
-// the next step's two in registers, packed: they are unpacked into the other
-// two LDS tiles after the step's barrier, and the loads of the step after that
-// go out behind them.
+// attn_impl.h's prefill kernels. A step has two tiles in LDS (K K or K V), the
+// next step's in registers, packed, and those of the step after on their way;
+// a step's tiles are unpacked into the other half of the LDS between the MFMAs
+// of the step before. Steps alternate between two halves of the code, so LDS
+// addresses and registers are fixed (an odd step is padded with one that only
+// moves data). The table entries of a chunk are one vector load, its granules'
+// offsets a lane each (scalar loads in the loop are waited for together with
+// the LDS reads: 397 us for four prompts of up to 2048 tokens with them and
+// one step's prefetch).
 //
 // SPLIT: the chunks of a row tile are dealt evenly to pq_splits workgroups; the
 // first folds its chunks and leaves the folded state as one record, the others
@@ -632,6 +651,7 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
   int r = int(quotient(blockIdx.x, m.by_heads));
   const int g = int(blockIdx.x) - r * a.num_kv_heads;
   int rtile = int(gridDim.y) - 1 - int(blockIdx.y);  // the longest row tiles first
+  if (a.pq_blocks == 0) r = turned(m, r, int(blockIdx.z * gridDim.y + blockIdx.y));
   if (a.pq_blocks > 0) {
     r = __builtin_amdgcn_readfirstlane(flat_block(a, a.pq_blocks - 1 - r, rtile));
     rtile = __builtin_amdgcn_readfirstlane(rtile);
@@ -666,44 +686,72 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
 
   auto live_lo = [&](int c) { return max(c * CT, t_lo); };
   auto live_hi = [&](int c) { return min(c * CT + CT, t_hi); };
-  // The steps of chunk c: phase 0 takes K tiles ta + 2 k, ta + 2 k + 1 (the last
-  // one twice where they are odd), phase 1 K and V of tile ta + k.
-  struct Step {
-    int c, phase, k, ta, n;  // (first live tile and live tiles of c)
+
+  // The stream of steps. Chunk c with n live tiles from ta has steps0(n) steps of
+  // phase 0 (K tiles 2 k, 2 k + 1) and steps1(n) of phase 1 (K and V of tile k),
+  // both even; tiles past the last are the last again.
+  auto steps0 = [](int n) { return 2 * ((n + 3) >> 2); };
+  auto steps1 = [](int n) { return 2 * ((n + 1) >> 1); };
+  // The staging cursor: the next step to load. A lane holds the byte offsets and
+  // limits (Pager) of granule `lane` of its chunk (32 granules).
+  int fc = c_lo, fphase = 0, fk = 0, fta = 0, fn = 1;
+  uint32_t oc_lo = 0, oc_hi = 0, os_lo = 0, os_hi = 0, lim_c = 0, lim_s = 0;
+  int ent = 0;  // the table entry of the lane's granule of chunk fc, then of chunk fc + 1
+  auto load_entry = [&](int c) { ent = a.bt[int64_t(r) * a.sbt + min((16 * pager.granule(32 * c + (lane & 31))) >> pager.ps_shift,
+                                                                    pager.max_blocks - 1)]; };
+  auto open_chunk = [&]() __attribute__((always_inline)) {
+    fta = live_lo(fc);
+    fn = live_hi(fc) - fta;
+    const int gq = pager.granule(32 * fc + (lane & 31));
+    const uint64_t oc = pager.offset(gq, ent, m.c_blk, m.c_slot, ch), os = pager.offset(gq, ent, m.s_blk, m.s_slot, sh);
+    oc_lo = uint32_t(oc);
+    oc_hi = uint32_t(oc >> 32);
+    os_lo = uint32_t(os);
+    os_hi = uint32_t(os >> 32);
+    lim_c = pager.limit(gq, m.c_slot) + 3 * (D / 8);
+    lim_s = pager.limit(gq, m.s_slot);
+    if (fc + 1 < c_hi) load_entry(fc + 1);
   };
-  auto first_step = [&](int c) { return Step{c, 0, 0, live_lo(c), live_hi(c) - live_lo(c)}; };
-  auto next = [&](Step s) {
-    ++s.k;
-    if (s.phase == 0) {
-      if (2 * s.k >= s.n) {
-        s.phase = 1;
-        s.k = 0;
+  auto advance = [&]() __attribute__((always_inline)) {
+    ++fk;
+    if (fphase == 0) {
+      if (fk >= steps0(fn)) {
+        fphase = 1;
+        fk = 0;
       }
-    } else if (s.k >= s.n) {
-      if (s.c + 1 < c_hi) s = first_step(s.c + 1);
-      else s.k = s.n - 1;  // past the end: the last step again
+    } else if (fk >= steps1(fn)) {
+      if (fc + 1 < c_hi) {
+        ++fc;
+        fphase = fk = 0;
+        open_chunk();
+      } else {
+        --fk;  // past the end: the last step again
+      }
     }
-    return s;
   };
-  auto tile0 = [&](const Step& s) { return s.ta + (s.phase ? s.k : 2 * s.k); };
-  auto tile1 = [&](const Step& s) { return s.ta + (s.phase ? s.k : min(2 * s.k + 1, s.n - 1)); };
 
   // Staging: the wave moves the tile's granule `wave`, lane l row l / 4, units
-  // l % 4. The table entries of a step are loaded a step before its tiles.
+  // l % 4.
   struct Staged {
     Units<D> u;
     Scales<D> s;
   };
   const int srow = 16 * wave + (lane >> 2);
   const uint32_t c_off = uint32_t(lane >> 2) * m.c_slot + (lane & 3) * (D / 8), s_off = uint32_t(lane >> 2) * m.s_slot;
-  auto fetch = [&](const uint8_t* codes, const uint8_t* scales, int t, int e) __attribute__((always_inline)) {
-    const int gq = pager.granule(4 * t + wave);
-    const uint8_t* cp = codes + pager.offset(gq, e, m.c_blk, m.c_slot, ch);
-    const uint8_t* sp = scales + pager.offset(gq, e, m.s_blk, m.s_slot, sh);
+  auto at_lane = [](uint32_t x, int l) { return uint32_t(__builtin_amdgcn_readlane(int(x), l)); };
+  auto fetch = [&](const uint8_t* codes, const uint8_t* scales, int k) __attribute__((always_inline)) {
+    const int l = 4 * (fta + min(k, fn - 1) - CT * fc) + wave;  // the granule in its chunk
+    const uint8_t* cp = codes + ((uint64_t(at_lane(oc_hi, l)) << 32) | at_lane(oc_lo, l));
+    const uint8_t* sp = scales + ((uint64_t(at_lane(os_hi, l)) << 32) | at_lane(os_lo, l));
     Staged x;
-    x.u = load_units<D>(cp + min(c_off, pager.limit(gq, m.c_slot) + 3 * (D / 8)));
-    x.s = load_scales<D>(sp + min(s_off, pager.limit(gq, m.s_slot)));
+    x.u = load_units<D>(cp + min(c_off, at_lane(lim_c, l)));
+    x.s = load_scales<D>(sp + min(s_off, at_lane(lim_s, l)));
     return x;
+  };
+  Staged r0[2], r1[2];  // by the step's parity
+  auto fetch0 = [&](Staged& x) __attribute__((always_inline)) { x = fetch(m.kc, m.ks, fphase ? fk : 2 * fk); };
+  auto fetch1 = [&](Staged& x) __attribute__((always_inline)) {
+    x = fetch(fphase ? m.vc : m.kc, fphase ? m.vs : m.ks, fphase ? fk : 2 * fk + 1);
   };
   unsigned kwr[QS], vwr[QS];
 #pragma unroll
@@ -711,32 +759,19 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
     kwr[j] = srow * L::ROWB + (((4 * j + (lane & 3)) ^ L::kswz(srow)) << 4);
     vwr[j] = srow * L::ROWB + (((4 * j + (lane & 3)) ^ L::vswz(srow)) << 4);
   }
-  auto put = [&](const Staged& x, unsigned char* tile, const unsigned (&at)[QS]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < QS; ++j)
-      lds_store16(tile + at[j], mx4::unpack8<DT>(x.u.w[j], mx4::scale_of<DT>(x.s.w[j / 4], j % 4)));
+  // unit j of a staged tile into LDS tile `tile` (of four)
+  auto put = [&](const Staged& x, int tile, const unsigned (&at)[QS], int j) __attribute__((always_inline)) {
+    lds_store16(lds + tile * L::TILEB + at[j], mx4::unpack8<DT>(x.u.w[j], mx4::scale_of<DT>(x.s.w[j / 4], j % 4)));
   };
-  auto tile_at = [&](int b, int j) { return lds + (2 * b + j) * L::TILEB; };
-  Staged r0, r1;
-  int e0 = 0, e1 = 0;
-  auto entries = [&](const Step& s) __attribute__((always_inline)) {
-    e0 = pager.entry(pager.granule(4 * tile0(s) + wave));
-    e1 = pager.entry(pager.granule(4 * tile1(s) + wave));
-  };
-  auto fetch_step = [&](const Step& s) __attribute__((always_inline)) {
-    r0 = fetch(m.kc, m.ks, tile0(s), e0);
-    r1 = fetch(s.phase ? m.vc : m.kc, s.phase ? m.vs : m.ks, tile1(s), e1);
-  };
-  auto put_step = [&](const Step& s, int b) __attribute__((always_inline)) {
-    put(r0, tile_at(b, 0), kwr);
-    if (s.phase) put(r1, tile_at(b, 1), vwr);  // uniform
-    else put(r1, tile_at(b, 1), kwr);
-  };
-  Step ahead{};  // the step whose tiles are in registers
   if (c_lo < c_hi) {
-    ahead = first_step(c_lo);
-    entries(ahead);
-    fetch_step(ahead);
+    load_entry(fc);
+    open_chunk();
+    fetch0(r0[0]);
+    fetch1(r1[0]);
+    advance();
+    fetch0(r0[1]);
+    fetch1(r1[1]);
+    advance();
   }
 
   // The lane's query row.
@@ -794,10 +829,9 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
     for (int b = 0; b < DBLK; ++b) wp[4 * b] = acc4{w[b][0], w[b][1], w[b][2], w[b][3]};
   };
 
-  int buf = 0;
   // The four score MFMA chains of a K tile; a chain's LDS reads go out before
-  // the chain before it is waited for.
-  auto scores_of = [&](const unsigned char* tile, auto&& fn) __attribute__((always_inline)) {
+  // the chain before it is waited for, and side(q) is done beside chain q.
+  auto scores_of = [&](const unsigned char* tile, auto&& side, auto&& fn) __attribute__((always_inline)) {
     u32x4 kf[2][QS];
     auto issue = [&](auto qc) __attribute__((always_inline)) {
       constexpr int q = decltype(qc)::value;
@@ -813,6 +847,7 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
 #pragma unroll
       for (int j = 0; j < QS; ++j) acc = TR::mma(kf[q & 1][j], qf[j], acc);
       accs[q & 1] = acc;
+      side(qc);
       if constexpr (q > 0) fn(std::integral_constant<int, q - 1>{}, accs[(q - 1) & 1]);
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -840,45 +875,73 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
   [[maybe_unused]] const float vlim = (BITS == 16 ? 32767.0f : 4194304.0f) / a.fxp_scale;
 
   if (c_lo < c_hi) {
-    put_step(ahead, 0);
-    Step after = next(ahead);
-    entries(after);
-    ahead = after;
-    fetch_step(ahead);
-    after = next(ahead);
-    entries(after);
-    // One step: publish its tiles, unpack the next step's, load the one after.
-    auto step_begin = [&]() __attribute__((always_inline)) {
-      lds_barrier();
-      put_step(ahead, buf ^ 1);
-      ahead = after;
-      fetch_step(ahead);
-      after = next(ahead);
-      entries(after);
+    // the first step's tiles (K K) to LDS; two more steps on their way
+#pragma unroll
+    for (int j = 0; j < QS; ++j) put(r0[0], 0, kwr, j);
+#pragma unroll
+    for (int j = 0; j < QS; ++j) put(r1[0], 1, kwr, j);
+    fetch0(r0[0]);
+    fetch1(r1[0]);
+    advance();
+    // a part of the units of the next step's first and second tile, beside the
+    // MFMAs of this one (parity P); VNEXT: its second tile is a V tile
+    constexpr int UPP = QS >= 4 ? QS / 4 : 1;
+    auto put0 = [&](auto pc, auto qc) __attribute__((always_inline)) {
+      constexpr int P = decltype(pc)::value, q = decltype(qc)::value;
+#pragma unroll
+      for (int j = q * UPP; j < (q + 1) * UPP && j < QS; ++j) put(r0[P ^ 1], 2 * (P ^ 1), kwr, j);
     };
+    auto put1 = [&](auto pc, auto qc, bool vnext) __attribute__((always_inline)) {
+      constexpr int P = decltype(pc)::value, q = decltype(qc)::value;
+#pragma unroll
+      for (int j = q * UPP; j < (q + 1) * UPP && j < QS; ++j) {
+        if constexpr (D == 64) put(r1[P ^ 1], 2 * (P ^ 1) + 1, vnext ? vwr : kwr, j);
+        else put(r1[P ^ 1], 2 * (P ^ 1) + 1, kwr, j);  // (the K swizzle is the V one)
+      }
+    };
+    auto put_all0 = [&](auto pc) __attribute__((always_inline)) { static_for<4>([&](auto qc) { put0(pc, qc); }); };
+    auto put_all1 = [&](auto pc, bool vnext) __attribute__((always_inline)) {
+      static_for<4>([&](auto qc) { put1(pc, qc, vnext); });
+    };
+    auto refill0 = [&](auto pc) __attribute__((always_inline)) { fetch0(r0[decltype(pc)::value ^ 1]); };
+    auto refill1 = [&](auto pc) __attribute__((always_inline)) {
+      fetch1(r1[decltype(pc)::value ^ 1]);
+      advance();
+    };
+
     for (int c = c_lo; c < c_hi; ++c) {
-      const int ta = live_lo(c), te = live_hi(c);
+      const int ta = live_lo(c), te = live_hi(c), n0 = steps0(te - ta), n1 = steps1(te - ta);
       float mx = -__builtin_inff(), mraw = -__builtin_inff();
       // phase 0: the chunk's row maxima
-      for (int t = ta; t < te; t += 2) {
-        step_begin();
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          if (t + j >= te) continue;  // uniform
-          if (FAST && tile_whole(t + j)) {
-            scores_of(tile_at(buf, j), [&](auto, const f32x4& acc) __attribute__((always_inline)) {
-              mraw = fmaxf(fmaxf(mraw, fmaxf(acc[0], acc[1])), fmaxf(acc[2], acc[3]));
-            });
-            if constexpr (CAP) mraw = fmaxf(mraw, -kFltMax);  // keys were seen
-          } else {
-            scores_of(tile_at(buf, j), [&](auto qc, const f32x4& acc) __attribute__((always_inline)) {
-              float sc[4];
-              chain_scores(acc, t + j, decltype(qc)::value, false, std::true_type{}, sc);
-              mx = fmaxf(fmaxf(mx, fmaxf(sc[0], sc[1])), fmaxf(sc[2], sc[3]));
-            });
-          }
+      auto max_tile = [&](int t, const unsigned char* tile, auto&& side) __attribute__((always_inline)) {
+        if (FAST && tile_whole(t)) {
+          scores_of(tile, side, [&](auto, const f32x4& acc) __attribute__((always_inline)) {
+            mraw = fmaxf(fmaxf(mraw, fmaxf(acc[0], acc[1])), fmaxf(acc[2], acc[3]));
+          });
+          if constexpr (CAP) mraw = fmaxf(mraw, -kFltMax);  // keys were seen
+        } else {
+          scores_of(tile, side, [&](auto qc, const f32x4& acc) __attribute__((always_inline)) {
+            float sc[4];
+            chain_scores(acc, t, decltype(qc)::value, false, std::true_type{}, sc);
+            mx = fmaxf(fmaxf(mx, fmaxf(sc[0], sc[1])), fmaxf(sc[2], sc[3]));
+          });
         }
-        buf ^= 1;
+      };
+      auto step0 = [&](auto pc, int k) __attribute__((always_inline)) {
+        constexpr int P = decltype(pc)::value;
+        const int t = ta + 2 * k;
+        const bool vnext = k + 1 >= n0;
+        lds_barrier();
+        if (t < te) max_tile(t, lds + 2 * P * L::TILEB, [&](auto qc) { put0(pc, qc); });
+        else put_all0(pc);
+        refill0(pc);
+        if (t + 1 < te) max_tile(t + 1, lds + (2 * P + 1) * L::TILEB, [&](auto qc) { put1(pc, qc, vnext); });
+        else put_all1(pc, vnext);
+        refill1(pc);
+      };
+      for (int k = 0; k < n0; k += 2) {
+        step0(std::integral_constant<int, 0>{}, k);
+        step0(std::integral_constant<int, 1>{}, k + 1);
       }
       if constexpr (FAST) {
         float m1 = __fmul_rn(mraw, a.scale_log2);
@@ -897,12 +960,23 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
       for (int b = 0; b < DBLK; ++b)
 #pragma unroll
         for (int e = 0; e < 4; ++e) wv[b][e] = 0;
-      for (int t = ta; t < te; ++t) {
-        step_begin();
+      auto step1 = [&](auto pc, int k) __attribute__((always_inline)) {
+        constexpr int P = decltype(pc)::value;
+        const int t = ta + k;
+        const bool vnext = k + 1 < n1;
+        lds_barrier();
+        if (t >= te) {  // uniform: a padding step
+          put_all0(pc);
+          refill0(pc);
+          put_all1(pc, vnext);
+          refill1(pc);
+          return;
+        }
         u32x4 pb[2];
         auto weights = [&](auto whole_tag) __attribute__((always_inline)) {
           constexpr bool WHOLE = decltype(whole_tag)::value;
-          scores_of(tile_at(buf, 0), [&](auto qc, const f32x4& acc) __attribute__((always_inline)) {
+          scores_of(lds + 2 * P * L::TILEB, [&](auto qc) { put0(pc, qc); }, [&](auto qc, const f32x4& acc)
+                    __attribute__((always_inline)) {
             constexpr int q = decltype(qc)::value, s = q >> 1, h = q & 1;
             float sc[4], w[4];
             chain_scores(acc, t, q, WHOLE, std::false_type{}, sc);
@@ -928,9 +1002,10 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
         };
         if (FAST && tile_whole(t)) weights(std::true_type{});
         else weights(std::false_type{});
+        refill0(pc);
 
         // d blocks, the next one's V reads before this one's MFMAs
-        const unsigned char* vt = tile_at(buf, 1);
+        const unsigned char* vt = lds + (2 * P + 1) * L::TILEB;
         u32x2 vr[2][2][2];
         auto issue_v = [&](auto bc) __attribute__((always_inline)) {
           constexpr int b = decltype(bc)::value;
@@ -949,6 +1024,7 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
 #pragma unroll
           for (int s = 0; s < 2; ++s)
             acc = TR::mma(u32x4{vr[b & 1][s][0][0], vr[b & 1][s][0][1], vr[b & 1][s][1][0], vr[b & 1][s][1][1]}, pb[s], acc);
+          if constexpr (b < 4) put1(pc, bc, vnext);
           if constexpr (FAST) {
             // block b - 1's terms while block b's MFMAs run
             accv[b] = acc;
@@ -959,6 +1035,7 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
           }
           __builtin_amdgcn_sched_barrier(0);
         });
+        refill1(pc);
         if constexpr (FAST) {
           vmax = absmax4(vmax, accv[DBLK - 1]);
           auto term = [&](float x) { return __float_as_uint(__builtin_fmaf(x, a.fxp_scale, kRoundF)); };
@@ -976,7 +1053,10 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
               }
           }
         }
-        buf ^= 1;
+      };
+      for (int k = 0; k < n1; k += 2) {
+        step1(std::integral_constant<int, 0>{}, k);
+        step1(std::integral_constant<int, 1>{}, k + 1);
       }
       if constexpr (FAST) {
         const uint32_t terms = uint32_t(te - ta) * kRound;
