@@ -33,17 +33,13 @@ Planned plan_mx4(int num_requests, int64_t num_tokens, int num_heads, int num_kv
   const int64_t wgs64 = std::max<int64_t>(cdiv(num_tokens * num_heads, PQROWS), 1);
   // chunks that a row's keys can touch
   const int64_t chunks = window > 0 ? std::min(slots, cdiv(int64_t(window) + max_query_len, TILE * CT) + 1) : slots;
-  int64_t s16 = 1, s64 = 1, per = 0;
+  int64_t s16 = 1, s64 = 1;
   if (requested >= 1) {
     s16 = s64 = std::min<int64_t>({int64_t(requested), slots, kMaxGridZ});
   } else {
     const bool only_long = r.p.rows64 && num_tokens == int64_t(num_requests) * max_query_len;
     if (chunks > 4 && wgs16 <= 8 * 256 && !only_long) {
-      s16 = std::min<int64_t>(window > 0 ? chunks : slots, 64);
-      if (window <= 0) {
-        per = cdiv(slots, s16);
-        s16 = cdiv(slots, per);
-      }
+      s16 = std::min<int64_t>(chunks, 64);
     }
     if (r.p.rows64 && chunks > 4 && wgs64 < 512) s64 = std::min(cdiv(2048, wgs64), chunks);
   }
@@ -69,7 +65,6 @@ Planned plan_mx4(int num_requests, int64_t num_tokens, int num_heads, int num_kv
   }
   r.p.splits = int(s16);
   r.p.pq_splits = int(s64);
-  r.p.chunks_per_split = s16 > 1 ? int(per) : 0;
   return r;
 }
 
@@ -195,6 +190,7 @@ extern "C" int fxpr_unified_attention_mx4(
   a.softcap_log2 = softcap_log2;
   a.fxp_scale = pow2f(frac_bits);
   a.fxp_inv = pow2f(-frac_bits);
+  m.vlim = (int_bits == 16 ? 32767.0f : 4194304.0f) * a.fxp_inv;
   hipStream_t st = as_stream(stream);
   return io_dtype == FXPR_DTYPE_BF16 ? run_mx4_bf16(m, plan.p, int_bits, num_requests, max_query_len, num_tokens, st)
                                      : run_mx4_f16(m, plan.p, int_bits, num_requests, max_query_len, num_tokens, st);

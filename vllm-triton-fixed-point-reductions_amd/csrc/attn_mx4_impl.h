@@ -36,6 +36,7 @@ struct Mx4Args {
   const uint8_t* ks;
   const uint8_t* vs;
   uint32_t c_blk, c_slot, c_head, s_blk, s_slot, s_head;  // bytes
+  float vlim;  // |x| below which the rounding constant quantises x (kRoundF)
   uint32_t by_group, by_heads, by_reqs;  // ceil(2^32 / x) of the group, kv heads and requests (see quotient)
 };
 
@@ -87,9 +88,8 @@ constexpr uint32_t kRound = 0x4B400000u;
 
 // Host plan of a launch.
 struct Mx4Plan {
-  int splits = 1;            // 16-row workgroups: splits of chunks_per_split chunks (0: dealt evenly)
-  int chunks_per_split = 0;
-  int pq_splits = 1;         // 64-row workgroups: key splits (chunks dealt evenly)
+  int splits = 1;            // key splits of the 16-row workgroups (every splits-th chunk)
+  int pq_splits = 1;         // of the 64-row workgroups (chunks dealt evenly)
   bool rows64 = false;       // requests of kPrefillRows rows or more in 64-row workgroups
   int tok_cap = 0;           // AttnArgs::tok_cap
 };
@@ -150,6 +150,35 @@ __device__ __forceinline__ u32x2 lds_load_tr8(const unsigned char* p) {
       u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(p)));
 }
 
+// Over the 16 lanes of a row, all of them getting the result: rotations within
+// the row as operands of the operation itself.
+template <int N> __device__ __forceinline__ int row_ror(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, 0x120 + N, 0xf, 0xf, false);
+}
+__device__ __forceinline__ float row16_max(float x) {
+  auto step = [](float v, int y) { return fmaxf(v, __uint_as_float(uint32_t(y))); };
+  x = step(x, row_ror<8>(int(__float_as_uint(x))));
+  x = step(x, row_ror<4>(int(__float_as_uint(x))));
+  x = step(x, row_ror<2>(int(__float_as_uint(x))));
+  return step(x, row_ror<1>(int(__float_as_uint(x))));
+}
+__device__ __forceinline__ uint32_t row16_sum(uint32_t x) {
+  x += uint32_t(row_ror<8>(int(x)));
+  x += uint32_t(row_ror<4>(int(x)));
+  x += uint32_t(row_ror<2>(int(x)));
+  return x + uint32_t(row_ror<1>(int(x)));
+}
+__device__ __forceinline__ uint64_t row16_sum(uint64_t x) {
+  auto turn = [](uint64_t v, auto n) {
+    constexpr int N = decltype(n)::value;
+    return (uint64_t(uint32_t(row_ror<N>(int(uint32_t(v >> 32))))) << 32) | uint32_t(row_ror<N>(int(uint32_t(v))));
+  };
+  x += turn(x, std::integral_constant<int, 8>{});
+  x += turn(x, std::integral_constant<int, 4>{});
+  x += turn(x, std::integral_constant<int, 2>{});
+  return x + turn(x, std::integral_constant<int, 1>{});
+}
+
 // A workgroup barrier that orders LDS but waits for no global load in flight.
 __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -175,6 +204,11 @@ struct Pager {
   // the table entry of (clamped) granule g
   __device__ __forceinline__ int entry(int g) const {
     return row[uint32_t(min((16 * g) >> ps_shift, max_blocks - 1))];
+  }
+  // the same per lane (a vector load), granules of a chunk: any beyond the
+  // sequence too (a clamped entry of the table row, never used)
+  __device__ __forceinline__ int entry_at(int g) const {
+    return reinterpret_cast<const int32_t*>((uint64_t)row)[uint32_t(min((16 * g) >> ps_shift, max_blocks - 1))];
   }
   __device__ __forceinline__ uint32_t block(int e) const { return uint32_t(e < 0 ? 0 : min(e, last_block)); }
   // byte offset of granule g's first row
@@ -207,195 +241,217 @@ template <class A> __device__ __forceinline__ Pager make_pager(const A& a, int r
 // barriers: the row maxima, and the waves' integer partial sums, which are
 // added in any order to the same bits (attn_impl.h's waves split them by d
 // instead). Loads run a phase ahead: a chunk's V goes out before its scores,
-// the next chunk's K before the weights.
+// the next chunk's K before the weights (with up to 4 rows behind them, where
+// the registers of a third workgroup per CU are worth more).
+//
+// NE: the workgroup has up to 4 NE rows (a decode step has as many as the GQA
+// group, often 4). The products are in the plain layout (query rows as the
+// MFMA's rows), row p as MFMA row 4 (p % 4) + p / 4: lane group kg then has rows
+// kg, kg + 4, .. in its result registers e = 0, 1, .., and with 4 rows only
+// e = 0 holds any. The softmax and the sums run over NE of the 4 registers (the
+// transposed layout of the 64-row kernel has no register to leave out: 102 us
+// for 64 requests up to 8192 keys, where the weights cross LDS here).
 //
 // FAST (the same bits): no softcap or ALiBi and a positive scale, so a score is
 // fl(dot * scale) and the chunk maximum fl(max(dot) * scale); sums by the
 // rounding constant (a weight is at most 1; a tile whose weighted V leaves the
 // constant's range is added exactly).
-template <int DT, int BITS, int D, bool SPLIT, bool FAST>
-__device__ __forceinline__ void rows16_body(const Mx4Args& m) {
+template <int BITS, int D, int MAXE> struct Rows16Lds {
+  using AccT = typename AccOf<BITS>::T;
+  // A wave's V stage: key row r at r * PITCH + (r / 8) * 32 bytes. The padding
+  // keeps the banks apart of the four rows (of 32 bytes each, two row groups of
+  // 8) that half a wave's transposing read takes and of the rows that its
+  // writes go to, and every d block and chunk is a constant away from one
+  // address (an XOR swizzle takes a register for each).
+  static constexpr int PITCH = Lds<D>::ROWB + 64;
+  static constexpr int STAGEB = 32 * PITCH + 3 * 32;
+  static constexpr int ROWS = 4 * MAXE;
+  static constexpr int PARTB = ROWS * D * int(sizeof(AccT));        // its partial sums, in the stage's place
+  static constexpr int WAVEB = STAGEB > PARTB ? STAGEB : PARTB;
+  static constexpr int VP = TILE + 8;                               // pitch of a row of weights
+  unsigned char stage[4][WAVEB];
+  uint16_t p[4][ROWS * VP];
+  float red_m[2][4][QROWS];  // (by the chunk's parity: no third barrier)
+  AccT red_d[4][QROWS];
+};
+
+// A workgroup's request and rows.
+struct Rows16 {
+  int r, g, q_start, q_len, seq_len, ctx, row0;
+};
+
+template <int DT, int BITS, int D, bool SPLIT, bool FAST, int NE, int MAXE>
+__device__ __forceinline__ void rows16_body(const Mx4Args& m, const Rows16& w, Rows16Lds<BITS, D, MAXE>& lds, int ent) {
   const AttnArgs& a = m.a;
   using TR = Traits<DT>;
   using T = typename TR::T;
   using AccT = typename AccOf<BITS>::T;
-  using L = Lds<D>;
+  using RL = Rows16Lds<BITS, D, MAXE>;
   constexpr int QS = D / 32, DBLK = D / 16, NT = CT / 4;
-  constexpr int VPT = D / 16;                      // accumulators per thread: 16 rows x D over 256 threads
-  constexpr int STAGEB = 32 * L::ROWB;             // the wave's V stage
-  constexpr int PARTB = QROWS * D * int(sizeof(AccT));  // the wave's partial sums, in the stage's place
-  constexpr int WAVEB = STAGEB > PARTB ? STAGEB : PARTB;
-  constexpr int EPC = 16 / int(sizeof(AccT));      // partial sums per 16-byte chunk
-  __shared__ __align__(16) unsigned char stage_all[4 * WAVEB];
-  __shared__ float red_m[2][4][QROWS];  // (by the chunk's parity: no third barrier)
-  __shared__ AccT red_d[4][QROWS];
-
+  constexpr int TPR = 64 / NE;       // threads per row in the sums over the waves
+  constexpr int VPT = NE * D / 64;   // elements of the row per thread
   const int tid = threadIdx.x, lane = tid & 63, kg = lane >> 4, i16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  unsigned char* stage = stage_all + wave * WAVEB;
-  const int slot_x = int(quotient(blockIdx.x, m.by_heads)), g = int(blockIdx.x) - slot_x * a.num_kv_heads;
-  const int split = blockIdx.z;
-  const int r = turned(m, slot_x, int(blockIdx.z * gridDim.y + blockIdx.y));
-  const int q_start = ((ConstI32)a.qsl)[r];
-  const int q_len = ((ConstI32)a.qsl)[r + 1] - q_start;
-  const int seq_len = ((ConstI32)a.seq_lens)[r];
-  const int ctx = seq_len - q_len;
-  const int rows_total = q_len * a.group;
-  const int row0 = blockIdx.y * QROWS;
-  if (row0 >= rows_total) return;                          // uniform
-  if (a.pq_rows > 0 && rows_total >= a.pq_rows) return;  // attn_mx4_rows64_kernel's request
-  auto ws_row = [&](int64_t token) { return a.tok_cap > 0 ? int64_t(r) * a.tok_cap + (token - q_start) : token; };
-
-  const int i_min = int(quotient(uint32_t(row0), m.by_group));
-  const int i_max = int(quotient(uint32_t(min(rows_total - 1, row0 + QROWS - 1)), m.by_group));
-  const int hi = a.causal ? min(seq_len, ctx + i_max + 1) : seq_len;
-  const int lo = a.window > 0 ? max(0, ctx + i_min - a.window + 1) : 0;
+  unsigned char* stage = lds.stage[wave];
+  uint16_t* pw = lds.p[wave];
+  auto ws_row = [&](int64_t token) { return a.tok_cap > 0 ? int64_t(w.r) * a.tok_cap + (token - w.q_start) : token; };
+  const int rows_total = w.q_len * a.group;
+  const int i_min = int(quotient(uint32_t(w.row0), m.by_group));
+  const int i_max = int(quotient(uint32_t(min(rows_total - 1, w.row0 + 4 * NE - 1)), m.by_group));
+  const int hi = a.causal ? min(w.seq_len, w.ctx + i_max + 1) : w.seq_len;
+  const int lo = a.window > 0 ? max(0, w.ctx + i_min - a.window + 1) : 0;
   const int t_lo = lo / TILE;
   const int t_hi = hi > lo ? (hi + TILE - 1) / TILE : t_lo;
   const int c_first = t_lo / CT;
   int c_end = t_hi > t_lo ? (t_hi + CT - 1) / CT : c_first;
   if constexpr (SPLIT) c_end = min(c_end, a.chunk_slots);
-  const int nch = max(0, c_end - c_first);
-  const int per = !SPLIT ? nch : a.chunks_per_split > 0 ? a.chunks_per_split : (nch + a.num_splits - 1) / a.num_splits;
-  const int c_lo = c_first + min(nch, (SPLIT ? split : 0) * per);
-  const int c_hi = min(c_first + nch, c_lo + per);
+  // this workgroup's chunks: every stride-th
+  const int stride = SPLIT ? a.num_splits : 1;
+  const int c_lo = c_first + (SPLIT ? int(blockIdx.z) : 0);
+  auto row_of = [&](int p) { return row_at(m, w.g, w.q_start, w.q_len, w.ctx, w.seq_len, w.row0 + p); };
 
-  // the thread's part of the sums: row tid / 16, elements VPT (tid % 16) ..
-  const RowInfo mine = row_at(m, g, q_start, q_len, ctx, seq_len, row0 + (tid >> 4));
-  const int my_d = VPT * (tid & 15);
-  if (SPLIT && split == 0 && (tid & 15) == 0 && mine.valid) {
-    int* cr = a.crange + 2 * (ws_row(mine.token) * a.num_heads + mine.head);
-    cr[0] = c_first;
-    cr[1] = c_first + nch;
+  if (SPLIT && blockIdx.z == 0 && tid < 4 * NE) {
+    const RowInfo ri = row_of(tid);
+    if (ri.valid) {
+      int* cr = a.crange + 2 * (ws_row(ri.token) * a.num_heads + ri.head);
+      cr[0] = c_first;
+      cr[1] = c_end;
+    }
   }
-  if (SPLIT && c_lo >= c_hi) return;  // uniform
+  if (SPLIT && c_lo >= c_end) return;  // uniform
 
-  const Pager pager = make_pager(a, r, seq_len);
-  const uint32_t ch = uint32_t(g) * m.c_head, sh = uint32_t(g) * m.s_head;
-
+  const Pager pager = make_pager(a, w.r, w.seq_len);
+  const uint32_t ch = uint32_t(w.g) * m.c_head, sh = uint32_t(w.g) * m.s_head;
   auto live_lo = [&](int c) { return max(c * CT, t_lo); };
   auto live_hi = [&](int c) { return min(c * CT + CT, t_hi); };
   // the wave's tile u (0, 1) of chunk c, moved onto a live one (whose loads are
   // in flight anyway) where it is none
   auto tile_of = [&](int c, int u) { return min(max(c * CT + wave + 4 * u, live_lo(c)), live_hi(c) - 1); };
 
-  int ent[NT][4];  // table entries of the granules of the wave's tiles
-  auto load_entries = [&](int c) __attribute__((always_inline)) {
+  // The byte offsets of a chunk's 32 granules, a lane each, from their table
+  // entries (loaded a chunk ahead; the first ones by the caller).
+  uint32_t oc_lo, oc_hi, os_lo, os_hi;
+  auto offsets = [&](int c) __attribute__((always_inline)) {
+    const int gq = 32 * c + (lane & 31);
+    const uint64_t oc = pager.offset(gq, ent, m.c_blk, m.c_slot, ch), os = pager.offset(gq, ent, m.s_blk, m.s_slot, sh);
+    oc_lo = uint32_t(oc);
+    oc_hi = uint32_t(oc >> 32);
+    os_lo = uint32_t(os);
+    os_hi = uint32_t(os >> 32);
+  };
+  auto at_lane = [](uint32_t x, int l) { return uint32_t(__builtin_amdgcn_readlane(int(x), l)); };
+  // A granule of the wave's tile: uniform bases and limits (Pager) of its code
+  // and scale rows.
+  struct Granule {
+    uint64_t c, s;
+    uint32_t cl, sl;
+  };
+  constexpr uint32_t kLastUnit = 3 * (D / 8);
+  auto granule = [&](int c, int t, int q) __attribute__((always_inline)) {
+    const int gq = pager.granule(4 * t + q), l = gq - 32 * c;
+    Granule x;
+    x.c = (uint64_t(at_lane(oc_hi, l)) << 32) | at_lane(oc_lo, l);
+    x.s = (uint64_t(at_lane(os_hi, l)) << 32) | at_lane(os_lo, l);
+    x.cl = pager.limit(gq, m.c_slot) + kLastUnit;
+    x.sl = pager.limit(gq, m.s_slot);
+    return x;
+  };
+  // K: lane (kg, i16) has row i16 of the granule, units kg. V: lane l has row
+  // l / 4, units l % 4.
+  const uint32_t kc_off = i16 * m.c_slot + kg * (D / 8), ks_off = i16 * m.s_slot;
+  const uint32_t vc_off = uint32_t(lane >> 2) * m.c_slot + (lane & 3) * (D / 8), vs_off = uint32_t(lane >> 2) * m.s_slot;
+  Units<D> kb[NT][4], vb[NT][4];
+  Scales<D> kbs[NT][4], vbs[NT][4];
+  auto load_k = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < NT; ++u)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) ent[u][q] = pager.entry(pager.granule(4 * tile_of(c, u) + q));
-  };
-
-  // K: MFMA row i16 of (s, h) is the tile's key 32 s + pi(i16, h), in granule
-  // 2 s + i16 / 8. (Offsets within a granule with the limits of Pager; a code
-  // offset holds the lane's unit too, and its limit the last unit.)
-  const bool up = i16 >= 8;
-  uint32_t kc_off[2], ks_off[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t in = uint32_t((8 * (i16 >> 2) + 4 * h + (i16 & 3)) & 15);
-    kc_off[h] = in * m.c_slot + kg * (D / 8);
-    ks_off[h] = in * m.s_slot;
-  }
-  constexpr uint32_t kLastUnit = 3 * (D / 8);
-  Units<D> kb[NT][4];
-  Scales<D> kbs[NT][4];
-  auto load_k = [&](int c) __attribute__((always_inline)) {
-#pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const int t = tile_of(c, u);
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int g0 = pager.granule(4 * t + 2 * s), g1 = pager.granule(4 * t + 2 * s + 1);
-        const uint64_t c0 = pager.offset(g0, ent[u][2 * s], m.c_blk, m.c_slot, ch);
-        const uint64_t c1 = pager.offset(g1, ent[u][2 * s + 1], m.c_blk, m.c_slot, ch);
-        const uint64_t s0 = pager.offset(g0, ent[u][2 * s], m.s_blk, m.s_slot, sh);
-        const uint64_t s1 = pager.offset(g1, ent[u][2 * s + 1], m.s_blk, m.s_slot, sh);
-        const uint8_t* cp = up ? m.kc + c1 : m.kc + c0;
-        const uint8_t* sp = up ? m.ks + s1 : m.ks + s0;
-        const uint32_t cl = (up ? pager.limit(g1, m.c_slot) : pager.limit(g0, m.c_slot)) + kLastUnit;
-        const uint32_t sl = up ? pager.limit(g1, m.s_slot) : pager.limit(g0, m.s_slot);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          kb[u][2 * s + h] = load_units<D>(cp + min(kc_off[h], cl));
-          kbs[u][2 * s + h] = load_scales<D>(sp + min(ks_off[h], sl));
-        }
+      for (int q = 0; q < 4; ++q) {
+        const Granule x = granule(c, tile_of(c, u), q);
+        kb[u][q] = load_units<D>(m.kc + x.c + min(kc_off, x.cl));
+        kbs[u][q] = load_scales<D>(m.ks + x.s + min(ks_off, x.sl));
       }
-    }
   };
-  // V: lane l of load q has row 16 q + l / 4 of the tile, units l % 4.
-  const uint32_t vc_off = uint32_t(lane >> 2) * m.c_slot + (lane & 3) * (D / 8), vs_off = uint32_t(lane >> 2) * m.s_slot;
-  Units<D> vb[NT][4];
-  Scales<D> vbs[NT][4];
   auto load_v = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const int t = tile_of(c, u);
+    for (int u = 0; u < NT; ++u)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int gq = pager.granule(4 * t + q);
-        const uint8_t* cp = m.vc + pager.offset(gq, ent[u][q], m.c_blk, m.c_slot, ch);
-        const uint8_t* sp = m.vs + pager.offset(gq, ent[u][q], m.s_blk, m.s_slot, sh);
-        vb[u][q] = load_units<D>(cp + min(vc_off, pager.limit(gq, m.c_slot) + kLastUnit));
-        vbs[u][q] = load_scales<D>(sp + min(vs_off, pager.limit(gq, m.s_slot)));
+        const Granule x = granule(c, tile_of(c, u), q);
+        vb[u][q] = load_units<D>(m.vc + x.c + min(vc_off, x.cl));
+        vbs[u][q] = load_scales<D>(m.vs + x.s + min(vs_off, x.sl));
       }
-    }
   };
-  if (c_lo < c_hi) {
-    load_entries(c_lo);
+  if (c_lo < c_end) {
+    offsets(c_lo);
     load_k(c_lo);
   }
 
-  // The lane's query row (a column of the score MFMAs).
-  const RowInfo me = row_at(m, g, q_start, q_len, ctx, seq_len, row0 + i16);
+  // Q as the A operand: lane row i16 is row i16 / 4 + 4 (i16 % 4).
   u32x4 qf[QS];
   {
-    const T* qbase = static_cast<const T*>(a.q) + me.token * a.sq_t + int64_t(me.head) * a.sq_h;
+    const RowInfo ri = row_of((i16 >> 2) + 4 * (i16 & 3));
+    const bool use = ri.valid && (i16 & 3) < NE;
+    const T* qbase = static_cast<const T*>(a.q) + ri.token * a.sq_t + int64_t(ri.head) * a.sq_h;
 #pragma unroll
     for (int j = 0; j < QS; ++j)
-      qf[j] = me.valid ? *reinterpret_cast<const u32x4*>(qbase + 32 * j + 8 * kg) : u32x4{0u, 0u, 0u, 0u};
+      qf[j] = use ? *reinterpret_cast<const u32x4*>(qbase + 32 * j + 8 * kg) : u32x4{0u, 0u, 0u, 0u};
   }
-  const int ks = me.valid ? me.kstart : 0x7fffffff;
-  const int ke = me.valid ? me.kend : 0;
-  const int qp = me.qpos;
-  const float slope = !FAST && a.alibi ? a.alibi[me.head] : 0.0f;
-  // (rows outside the request see no key and are never stored: a tile counts as
-  // whole when every row of the request sees all of it)
+  // The lane's rows kg + 4 e of the results: visible keys (none outside the request).
+  int ks[NE], ke[NE], qp[NE];
+  float slope[NE];
+  int all_lo = 0, all_hi = 0x7fffffff;  // keys that every row of the lane sees
+#pragma unroll
+  for (int e = 0; e < NE; ++e) {
+    const RowInfo ri = row_of(kg + 4 * e);
+    ks[e] = ri.valid ? ri.kstart : 0x7fffffff;
+    ke[e] = ri.valid ? ri.kend : 0;
+    qp[e] = ri.qpos;
+    slope[e] = !FAST && a.alibi ? a.alibi[ri.head] : 0.0f;
+    // (rows outside the request see no key and are never stored: they count as
+    // seeing everything)
+    all_lo = max(all_lo, ri.valid ? ri.kstart : 0);
+    all_hi = min(all_hi, ri.valid ? ri.kend : 0x7fffffff);
+  }
   auto tile_whole = [&](int t) -> bool {
-    return __builtin_amdgcn_ballot_w64(me.valid && !(ks <= t * TILE && t * TILE + TILE <= ke)) == 0;
+    return __builtin_amdgcn_ballot_w64(!(all_lo <= t * TILE && t * TILE + TILE <= all_hi)) == 0;
   };
 
-  // LDS addresses of the V stage: the chunk slots the lane writes (row lane / 4;
-  // the second granule is 16 rows on, which the swizzle ignores), and its
-  // transposing reads (keys 8 kg + j / 4 + 4 h, columns 4 (j % 4) of d block 0;
-  // d block db is at ^ (db << 5)).
-  unsigned vwr[QS], vrd[2];
-#pragma unroll
-  for (int j = 0; j < QS; ++j)
-    vwr[j] = (lane >> 2) * L::ROWB + (((4 * j + (lane & 3)) ^ L::vswz(lane >> 2)) << 4);
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int rr = 8 * kg + (i16 >> 2) + 4 * h;
-    vrd[h] = rr * L::ROWB + ((((i16 & 3) >> 1) ^ L::vswz(rr)) << 4) + (i16 & 1) * 8;
-  }
+  // LDS addresses of the V stage: where the lane writes (row lane / 4, chunk
+  // lane % 4; chunk 4 j + lane % 4 is 64 j on, the second granule 16 rows), and
+  // its transposing reads (keys 8 kg + j / 4 + 4 h, columns 4 (j % 4) of d block
+  // 0, j = lane % 16; d block b is 32 b on).
+  unsigned char* vst = stage + (lane >> 2) * RL::PITCH + (lane >> 5) * 32 + (lane & 3) * 16;
+  const unsigned char* vld = stage + (8 * kg + (i16 >> 2)) * RL::PITCH + kg * 32 + (i16 & 3) * 8;
+  // the weights' rows: written by result rows, read as the A operand's
+  uint16_t* pst = pw + kg * RL::VP + i16;
+  const uint16_t* pld = pw + ((i16 >> 2) + 4 * ((i16 & 3) < NE ? (i16 & 3) : 0)) * RL::VP + 8 * kg;
 
-  float M = -__builtin_inff();  // the thread's row, folded
+  // the thread's part of the sums: row tid / TPR, elements my_d ..
+  const int my_row = tid / TPR, my_d = VPT * (tid % TPR);
+  float M = -__builtin_inff();
   AccT Dn = 0, W[VPT];
 #pragma unroll
   for (int v = 0; v < VPT; ++v) W[v] = 0;
-  [[maybe_unused]] const float vlim = (BITS == 16 ? 32767.0f : 4194304.0f) / a.fxp_scale;
 
-  if (c_lo < c_hi) {
-    for (int c = c_lo;; ++c) {
+  if (c_lo < c_end) {
+    for (int c = c_lo, par = 0;; c += stride, par ^= 1) {
       const int ta = live_lo(c), te = live_hi(c);
+      const bool more = c + stride < c_end;  // uniform
       load_v(c);
-      if (c + 1 < c_hi) load_entries(c + 1);
+      if (more) ent = pager.entry_at(32 * (c + stride) + (lane & 31));
+      auto next_k = [&]() __attribute__((always_inline)) {
+        if (more) {
+          offsets(c + stride);
+          load_k(c + stride);
+        }
+      };
 
-      // the wave's tiles: dots (FAST) or scores, for the lane's row and keys
-      // 32 s + 8 kg + 4 h + e, -inf where masked
-      f32x4 sc[NT][4];
-      float mx = -__builtin_inff();
+      // the wave's tiles: dots (FAST) or scores, for the lane's rows and keys
+      // 16 q + i16 of the tile, -inf where masked
+      float sc[NT][4][NE], mx[NE];
+#pragma unroll
+      for (int e = 0; e < NE; ++e) mx[e] = -__builtin_inff();
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
         const int t = c * CT + wave + 4 * u;
@@ -405,187 +461,165 @@ __device__ __forceinline__ void rows16_body(const Mx4Args& m) {
           f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < QS; ++j)
-            acc = TR::mma(mx4::unpack8<DT>(kb[u][q].w[j], mx4::scale_of<DT>(kbs[u][q].w[j / 4], j % 4)), qf[j], acc);
-          if constexpr (!FAST) {
-            const int key0 = t * TILE + 32 * (q >> 1) + 8 * kg + 4 * (q & 1);
+            acc = TR::mma(qf[j], mx4::unpack8<DT>(kb[u][q].w[j], mx4::scale_of<DT>(kbs[u][q].w[j / 4], j % 4)), acc);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float x = __fmul_rn(acc[e], a.scale_log2);
+          for (int e = 0; e < NE; ++e) {
+            float x = acc[e];
+            if constexpr (!FAST) {
+              x = __fmul_rn(x, a.scale_log2);
               if (a.softcap_log2 > 0.0f) x = softcapped(x, a.softcap_log2);
-              if (a.alibi) x = x + slope * static_cast<float>(key0 + e - qp);
-              acc[e] = x;
+              if (a.alibi) x = x + slope[e] * static_cast<float>(t * TILE + 16 * q + i16 - qp[e]);
             }
+            sc[u][q][e] = x;
           }
-          sc[u][q] = acc;
         }
         if (!live || !tile_whole(t)) {  // uniform
-          const int k0 = t * TILE + 8 * kg;
 #pragma unroll
           for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int key = k0 + 32 * (q >> 1) + 4 * (q & 1) + e;
-              sc[u][q][e] = (live && key >= ks && key < ke) ? sc[u][q][e] : -__builtin_inff();
+            for (int e = 0; e < NE; ++e) {
+              const int key = t * TILE + 16 * q + i16;
+              sc[u][q][e] = (live && key >= ks[e] && key < ke[e]) ? sc[u][q][e] : -__builtin_inff();
             }
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) mx = fmaxf(fmaxf(mx, fmaxf(sc[u][q][0], sc[u][q][1])), fmaxf(sc[u][q][2], sc[u][q][3]));
+        for (int e = 0; e < NE; ++e)
+          mx[e] = fmaxf(fmaxf(mx[e], fmaxf(sc[u][0][e], sc[u][1][e])), fmaxf(sc[u][2][e], sc[u][3][e]));
       }
-      if (c + 1 < c_hi) load_k(c + 1);
+      if constexpr (MAXE > 1) next_k();
 
-      // the chunk's row maxima: the row's four lanes, then the waves
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      if constexpr (FAST) mx = __fmul_rn(mx, a.scale_log2);
-      float(&rm)[4][QROWS] = red_m[c & 1];
-      if (kg == 0) rm[wave][i16] = mx;
+      // the chunk's row maxima: the row's 16 lanes, then the waves
+      float(&rm)[4][QROWS] = lds.red_m[par];
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        mx[e] = row16_max(mx[e]);
+        if constexpr (FAST) mx[e] = __fmul_rn(mx[e], a.scale_log2);
+        if (i16 == 0) rm[wave][kg + 4 * e] = mx[e];
+      }
       lds_barrier();
-      mx = fmaxf(fmaxf(rm[0][i16], rm[1][i16]), fmaxf(rm[2][i16], rm[3][i16]));
-      const float mrow = mx != -__builtin_inff() ? mx : 0.0f;  // no key: pin to 0
+      float mrow[NE];
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        const int p = kg + 4 * e;
+        const float x = fmaxf(fmaxf(rm[0][p], rm[1][p]), fmaxf(rm[2][p], rm[3][p]));
+        mrow[e] = x != -__builtin_inff() ? x : 0.0f;  // no key: pin to 0
+      }
 
       // weights and weighted V of the wave's tiles. FAST: the sums carry
       // kRound per added term, taken out below.
-      AccT den = 0;
-      AccT wv[DBLK][4];
+      AccT den[NE], wv[DBLK][NE];
 #pragma unroll
-      for (int b = 0; b < DBLK; ++b)
+      for (int e = 0; e < NE; ++e) {
+        den[e] = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) wv[b][e] = 0;
+        for (int b = 0; b < DBLK; ++b) wv[b][e] = 0;
+      }
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
         const int t = c * CT + wave + 4 * u;
         if (t >= ta && t < te) {  // uniform
+          lds_wave_order();
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < NE; ++e) {
+              const float x = FAST ? __fmul_rn(sc[u][q][e], a.scale_log2) : sc[u][q][e];
+              const float wt = __builtin_amdgcn_exp2f(x - mrow[e]);
+              if constexpr (FAST)  // (the maximum: NaN counts as 0)
+                den[e] = AccT(uint32_t(den[e]) + __float_as_uint(fmaxf(__builtin_fmaf(wt, a.fxp_scale, kRoundF), kRoundF)));
+              else
+                den[e] = wadd<BITS>(den[e], quant<BITS>(__fmul_rn(wt, a.fxp_scale)));
+              pst[4 * e * RL::VP + 16 * q] = FAST ? uint16_t(p_pack2<DT>(wt, wt)) : Io<DT>::store(wt);
+            }
           f32x4 acc[DBLK];
 #pragma unroll
           for (int b = 0; b < DBLK; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            u32x4 pb;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float x = FAST ? __fmul_rn(sc[u][2 * s + h][e], a.scale_log2) : sc[u][2 * s + h][e];
-                w[e] = __builtin_amdgcn_exp2f(x - mrow);
-              }
-              if constexpr (FAST) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)  // (the maximum: NaN counts as 0)
-                  den = AccT(uint32_t(den) + __float_as_uint(fmaxf(__builtin_fmaf(w[e], a.fxp_scale, kRoundF), kRoundF)));
-                pb[2 * h] = p_pack2<DT>(w[0], w[1]);
-                pb[2 * h + 1] = p_pack2<DT>(w[2], w[3]);
-              } else {
-                uint32_t p16[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  den = wadd<BITS>(den, quant<BITS>(__fmul_rn(w[e], a.fxp_scale)));
-                  p16[e] = Io<DT>::store(w[e]);
-                }
-                pb[2 * h] = p16[0] | (p16[1] << 16);
-                pb[2 * h + 1] = p16[2] | (p16[3] << 16);
-              }
-            }
-            lds_wave_order();
 #pragma unroll
             for (int q = 0; q < 2; ++q)
 #pragma unroll
               for (int j = 0; j < QS; ++j)
-                lds_store16(stage + vwr[j] + q * 16 * L::ROWB,
+                lds_store16(vst + (q * (16 * RL::PITCH + 64) + 64 * j),
                             mx4::unpack8<DT>(vb[u][2 * s + q].w[j],
                                              mx4::scale_of<DT>(vbs[u][2 * s + q].w[j / 4], j % 4)));
             lds_wave_order();
+            const u32x4 pa = *reinterpret_cast<const u32x4*>(pld + 32 * s);
 #pragma unroll
             for (int b = 0; b < DBLK; ++b) {
-              const u32x2 lo2 = lds_load_tr8(stage + (vrd[0] ^ (b << 5)));
-              const u32x2 hi2 = lds_load_tr8(stage + (vrd[1] ^ (b << 5)));
-              acc[b] = TR::mma(u32x4{lo2[0], lo2[1], hi2[0], hi2[1]}, pb, acc[b]);
+              const u32x2 lo2 = lds_load_tr8(vld + 32 * b);
+              const u32x2 hi2 = lds_load_tr8(vld + (4 * RL::PITCH + 32 * b));
+              acc[b] = TR::mma(pa, u32x4{lo2[0], lo2[1], hi2[0], hi2[1]}, acc[b]);
             }
+            lds_wave_order();
           }
           if constexpr (FAST) {
-            den = AccT(uint32_t(den) - 16u * kRound);
+            auto term = [&](float x) { return __float_as_uint(__builtin_fmaf(x, a.fxp_scale, kRoundF)); };
             float vmax = 0.0f;
 #pragma unroll
-            for (int b = 0; b < DBLK; ++b) {
-              vmax = absmax4(vmax, acc[b]);
+            for (int e = 0; e < NE; ++e) {
+              den[e] = AccT(uint32_t(den[e]) - 4u * kRound);
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                wv[b][e] = AccT(uint32_t(wv[b][e]) + __float_as_uint(__builtin_fmaf(acc[b][e], a.fxp_scale, kRoundF)));
+              for (int b = 0; b < DBLK; ++b) {
+                vmax = __builtin_elementwise_maximum(vmax, __builtin_fabsf(acc[b][e]));
+                wv[b][e] = AccT(uint32_t(wv[b][e]) + term(acc[b][e]));
+              }
             }
-            if (__builtin_amdgcn_ballot_w64(!(vmax < vlim)) != 0) {  // uniform: out of the constant's range
+            if (__builtin_amdgcn_ballot_w64(!(vmax < m.vlim)) != 0) {  // uniform: out of the constant's range
 #pragma unroll
               for (int b = 0; b < DBLK; ++b)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const uint32_t without =
-                      uint32_t(wv[b][e]) - __float_as_uint(__builtin_fmaf(acc[b][e], a.fxp_scale, kRoundF));
-                  wv[b][e] = AccT(uint32_t(wadd<BITS>(AccT(without), quant<BITS>(__fmul_rn(acc[b][e], a.fxp_scale)))) + kRound);
+                for (int e = 0; e < NE; ++e) {
+                  const AccT without = AccT(uint32_t(wv[b][e]) - term(acc[b][e]));
+                  wv[b][e] = AccT(uint32_t(wadd<BITS>(without, quant<BITS>(__fmul_rn(acc[b][e], a.fxp_scale)))) + kRound);
                 }
             }
           } else {
 #pragma unroll
             for (int b = 0; b < DBLK; ++b)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
+              for (int e = 0; e < NE; ++e)
                 wv[b][e] = wadd<BITS>(wv[b][e], quant<BITS>(__fmul_rn(acc[b][e], a.fxp_scale)));
           }
         }
       }
 
-      // the waves' partial sums to LDS, rows of D with 16-byte chunk x of row i
-      // at x ^ i: lane (kg, row) holds d = 16 b + 4 kg + e
-      den = wadd<BITS>(den, __shfl_xor(den, 16, 64));
-      den = wadd<BITS>(den, __shfl_xor(den, 32, 64));
-      if (kg == 0) red_d[wave][i16] = den;
-      lds_wave_order();
-      if (me.valid) {
-        typedef AccT accc __attribute__((ext_vector_type(EPC)));
-        accc* p = reinterpret_cast<accc*>(stage) + i16 * (D / EPC);
+      if constexpr (MAXE == 1) next_k();
+
+      // the waves' partial sums to LDS, rows of D, the 16-element group x of row p
+      // at x ^ (p % 4): lane (kg, i16) holds elements 16 b + i16 of its rows
 #pragma unroll
-        for (int b = 0; b < DBLK; ++b)
+      for (int e = 0; e < NE; ++e) {
+        den[e] = AccT(row16_sum(typename std::make_unsigned<AccT>::type(den[e])));
+        if (i16 == 0) lds.red_d[wave][kg + 4 * e] = den[e];
+        AccT* p = reinterpret_cast<AccT*>(stage) + (kg + 4 * e) * D + i16;
 #pragma unroll
-          for (int x = 0; x < 4 / EPC; ++x) {
-            accc v;
-#pragma unroll
-            for (int e = 0; e < EPC; ++e) v[e] = wv[b][x * EPC + e];
-            p[((4 * b + kg) * (4 / EPC) + x) ^ i16] = v;
-          }
+        for (int b = 0; b < DBLK; ++b) p[16 * (b ^ kg)] = wv[b][e];
       }
       lds_barrier();
+      const RowInfo mine = row_of(my_row);
       if (mine.valid) {
-        typedef AccT accc __attribute__((ext_vector_type(EPC)));
-        const int row = tid >> 4;
-        const AccT cd = wadd<BITS>(wadd<BITS>(red_d[0][row], red_d[1][row]), wadd<BITS>(red_d[2][row], red_d[3][row]));
-        const float cm = fmaxf(fmaxf(rm[0][row], rm[1][row]), fmaxf(rm[2][row], rm[3][row]));
+        const AccT cd = wadd<BITS>(wadd<BITS>(lds.red_d[0][my_row], lds.red_d[1][my_row]),
+                                   wadd<BITS>(lds.red_d[2][my_row], lds.red_d[3][my_row]));
+        const float cm = fmaxf(fmaxf(rm[0][my_row], rm[1][my_row]), fmaxf(rm[2][my_row], rm[3][my_row]));
+        const int at = my_row * D + (my_d ^ ((my_row & 3) << 4));
         AccT cw[VPT];
 #pragma unroll
-        for (int x = 0; x < VPT / EPC; ++x) {
-          const int at = row * (D / EPC) + ((my_d / EPC + x) ^ row);
-          accc v[4];
+        for (int v = 0; v < VPT; ++v) {
+          cw[v] = 0;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) v[w] = reinterpret_cast<const accc*>(stage_all + w * WAVEB)[at];
-#pragma unroll
-          for (int e = 0; e < EPC; ++e)
-            cw[x * EPC + e] = wadd<BITS>(wadd<BITS>(v[0][e], v[1][e]), wadd<BITS>(v[2][e], v[3][e]));
-        }
-        if constexpr (FAST) {
-#pragma unroll
-          for (int v = 0; v < VPT; ++v) cw[v] = AccT(uint32_t(cw[v]) - uint32_t(te - ta) * kRound);
+          for (int x = 0; x < 4; ++x) cw[v] = wadd<BITS>(cw[v], reinterpret_cast<const AccT*>(lds.stage[x])[at + v]);
+          if constexpr (FAST) cw[v] = AccT(uint32_t(cw[v]) - uint32_t(te - ta) * kRound);
         }
         if constexpr (SPLIT) {
           const int64_t slot = (ws_row(mine.token) * a.num_heads + mine.head) * a.chunk_slots + c;
-          if ((tid & 15) == 0) {
+          if (my_d == 0) {
             a.pmax[slot] = cm;
             static_cast<AccT*>(a.den_ws)[slot] = cd;
           }
           AccT* wp = static_cast<AccT*>(a.wv_ws) + slot * D + my_d;
 #pragma unroll
-          for (int x = 0; x < VPT / EPC; ++x) {
-            accc v;
-#pragma unroll
-            for (int e = 0; e < EPC; ++e) v[e] = cw[x * EPC + e];
-            reinterpret_cast<accc*>(wp)[x] = v;
-          }
+          for (int v = 0; v < VPT; ++v) wp[v] = cw[v];
         } else if (cm != -__builtin_inff()) {
           float Mn, fa, fb;
           merge_factors(M, cm, Mn, fa, fb);
@@ -597,11 +631,12 @@ __device__ __forceinline__ void rows16_body(const Mx4Args& m) {
       }
       // (the next chunk's first barrier stands between these reads and the
       // next writes of the stages and of red_d)
-      if (c + 1 >= c_hi) break;
+      if (!more) break;
     }
   }
 
   if constexpr (!SPLIT) {
+    const RowInfo mine = row_of(my_row);
     if (mine.valid) {
       const float den_f = fmaxf(acc_f32<BITS>(Dn, a.fxp_inv), 1.0e-6f);
       T* o = static_cast<T*>(a.o) + mine.token * a.so_t + int64_t(mine.head) * a.so_h + my_d;
@@ -611,9 +646,48 @@ __device__ __forceinline__ void rows16_body(const Mx4Args& m) {
   }
 }
 
-template <int DT, int BITS, int D, bool SPLIT, bool FAST>
-__global__ __launch_bounds__(kThreads, D == 256 || BITS == 64 ? 1 : 2) void attn_mx4_rows16_kernel(Mx4Args m) {
-  rows16_body<DT, BITS, D, SPLIT, FAST>(m);
+// MAXE: no request of the launch has more than 4 MAXE rows in a tile (1: decode
+// steps of a group of up to 4). Workgroups per CU that the registers are held to:
+// with up to 4 rows three, whose loads in flight hide each other's start (two
+// dependent round trips: the request's bounds beside the table entries, then K
+// and V), else two.
+template <int BITS, int D, int MAXE> constexpr int rows16_wgs() {
+  return BITS == 64 || D == 256 ? 1 : MAXE == 1 ? 3 : 2;
+}
+
+template <int DT, int BITS, int D, bool SPLIT, bool FAST, int MAXE>
+__global__ __launch_bounds__(kThreads, (rows16_wgs<BITS, D, MAXE>())) void attn_mx4_rows16_kernel(Mx4Args m) {
+  __shared__ __align__(16) Rows16Lds<BITS, D, MAXE> lds;
+  const AttnArgs& a = m.a;
+  const int lane = threadIdx.x & 63;
+  const int slot_x = int(quotient(blockIdx.x, m.by_heads));
+  Rows16 w;
+  w.g = int(blockIdx.x) - slot_x * a.num_kv_heads;
+  w.r = turned(m, slot_x, int(blockIdx.z * gridDim.y + blockIdx.y));
+  // the table entries of the first chunk, where it follows from the launch
+  // alone, beside the request's bounds
+  Pager pg = make_pager(a, w.r, 0);
+  int ent = pg.entry_at(32 * (SPLIT ? int(blockIdx.z) : 0) + (lane & 31));
+  w.q_start = ((ConstI32)a.qsl)[w.r];
+  w.q_len = ((ConstI32)a.qsl)[w.r + 1] - w.q_start;
+  w.seq_len = ((ConstI32)a.seq_lens)[w.r];
+  w.ctx = w.seq_len - w.q_len;
+  const int rows_total = w.q_len * a.group;
+  w.row0 = blockIdx.y * (MAXE == 4 ? QROWS : 4 * MAXE);
+  if (w.row0 >= rows_total) return;                        // uniform
+  if (a.pq_rows > 0 && rows_total >= a.pq_rows) return;  // attn_mx4_rows64_kernel's request
+  if (a.window > 0) {
+    const int i_min = int(quotient(uint32_t(w.row0), m.by_group));
+    const int c = max(0, w.ctx + i_min - a.window + 1) / (TILE * CT) + (SPLIT ? int(blockIdx.z) : 0);
+    ent = pg.entry_at(32 * c + (lane & 31));
+  }
+  if constexpr (MAXE == 1) {
+    rows16_body<DT, BITS, D, SPLIT, FAST, 1>(m, w, lds, ent);
+  } else {
+    // (a batch of decode steps beside a few short prompts)
+    if (rows_total - w.row0 <= 4) rows16_body<DT, BITS, D, SPLIT, FAST, 1>(m, w, lds, ent);
+    else rows16_body<DT, BITS, D, SPLIT, FAST, MAXE>(m, w, lds, ent);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -872,7 +946,6 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
       sc[e] = (whole || (key0 + e >= ks && key0 + e < ke)) ? x : -__builtin_inff();
     }
   };
-  [[maybe_unused]] const float vlim = (BITS == 16 ? 32767.0f : 4194304.0f) / a.fxp_scale;
 
   if (c_lo < c_hi) {
     // the first step's tiles (K K) to LDS; two more steps on their way
@@ -1043,7 +1116,7 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
           for (int b = 0; b < DBLK; ++b)
 #pragma unroll
             for (int e = 0; e < 4; ++e) wv[b][e] = AccT(uint32_t(wv[b][e]) + term(accv[b][e]));
-          if (__builtin_amdgcn_ballot_w64(!(vmax < vlim)) != 0) {  // uniform: out of the constant's range
+          if (__builtin_amdgcn_ballot_w64(!(vmax < m.vlim)) != 0) {  // uniform: out of the constant's range
 #pragma unroll
             for (int b = 0; b < DBLK; ++b)
 #pragma unroll
@@ -1329,21 +1402,25 @@ template <int DT, int BITS, int D, bool SPLIT> int launch_rows64(const Mx4Args& 
   return launch_rows64<DT, BITS, D, SPLIT, false, false>(m, grid, st);
 }
 
-template <int DT, int BITS, int D, bool SPLIT> void launch_rows16(const Mx4Args& m, dim3 grid, hipStream_t st) {
+template <int DT, int BITS, int D, bool SPLIT, int MAXE> void launch_rows16(const Mx4Args& m, dim3 grid, hipStream_t st) {
   if constexpr (BITS != 64) {
     if (fast_of<BITS>(m.a) && !(m.a.softcap_log2 > 0.0f)) {
-      attn_mx4_rows16_kernel<DT, BITS, D, SPLIT, true><<<grid, kThreads, 0, st>>>(m);
+      attn_mx4_rows16_kernel<DT, BITS, D, SPLIT, true, MAXE><<<grid, kThreads, 0, st>>>(m);
       return;
     }
   }
-  attn_mx4_rows16_kernel<DT, BITS, D, SPLIT, false><<<grid, kThreads, 0, st>>>(m);
+  attn_mx4_rows16_kernel<DT, BITS, D, SPLIT, false, MAXE><<<grid, kThreads, 0, st>>>(m);
+}
+template <int DT, int BITS, int D> void launch_rows16(const Mx4Args& m, dim3 grid, bool split, int max_e, hipStream_t st) {
+  if (max_e == 1) split ? launch_rows16<DT, BITS, D, true, 1>(m, grid, st) : launch_rows16<DT, BITS, D, false, 1>(m, grid, st);
+  else if (max_e == 2) split ? launch_rows16<DT, BITS, D, true, 2>(m, grid, st) : launch_rows16<DT, BITS, D, false, 2>(m, grid, st);
+  else split ? launch_rows16<DT, BITS, D, true, 4>(m, grid, st) : launch_rows16<DT, BITS, D, false, 4>(m, grid, st);
 }
 
 template <int DT, int BITS, int D>
 int launch_mx4(Mx4Args m, const Mx4Plan& p, int num_requests, int max_query_len, int64_t num_tokens, hipStream_t st) {
   AttnArgs& a = m.a;
   a.num_splits = p.splits;
-  a.chunks_per_split = p.chunks_per_split;
   a.pq_splits = p.pq_splits;
   a.tok_cap = p.tok_cap;
   const int64_t max_rows = int64_t(max_query_len > 1 ? max_query_len : 1) * a.group;
@@ -1366,11 +1443,10 @@ int launch_mx4(Mx4Args m, const Mx4Plan& p, int num_requests, int max_query_len,
     if (e) return e;
   }
   const dim3 grid(unsigned(num_requests * a.num_kv_heads), unsigned(qtiles), unsigned(p.splits));
-  if (!split) {
-    launch_rows16<DT, BITS, D, false>(m, grid, st);
-    return launch_status();
-  }
-  launch_rows16<DT, BITS, D, true>(m, grid, st);
+  // (rows of the longest request that these workgroups can get)
+  const int64_t short_rows = p.rows64 ? kPrefillRows - 1 : max_rows;
+  launch_rows16<DT, BITS, D>(m, grid, split, short_rows <= 4 ? 1 : short_rows <= 8 ? 2 : 4, st);
+  if (!split) return launch_status();
   const int64_t ws_rows = a.tok_cap > 0 ? int64_t(num_requests) * a.tok_cap : num_tokens;
   const int64_t rows = ws_rows * a.num_heads;
   if (rows < kWideRows && a.chunk_slots > kWideChunks)
