@@ -372,15 +372,13 @@ __device__ __forceinline__ void rows16_body(const Mx4Args& m, const Rows16& w, R
         kbs[u][q] = load_scales<D>(m.ks + x.s + min(ks_off, x.sl));
       }
   };
-  auto load_v = [&](int c) __attribute__((always_inline)) {
+  auto load_v = [&](int c, int u) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < NT; ++u)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const Granule x = granule(c, tile_of(c, u), q);
-        vb[u][q] = load_units<D>(m.vc + x.c + min(vc_off, x.cl));
-        vbs[u][q] = load_scales<D>(m.vs + x.s + min(vs_off, x.sl));
-      }
+    for (int q = 0; q < 4; ++q) {
+      const Granule x = granule(c, tile_of(c, u), q);
+      vb[u][q] = load_units<D>(m.vc + x.c + min(vc_off, x.cl));
+      vbs[u][q] = load_scales<D>(m.vs + x.s + min(vs_off, x.sl));
+    }
   };
   if (c_lo < c_end) {
     offsets(c_lo);
@@ -438,7 +436,8 @@ __device__ __forceinline__ void rows16_body(const Mx4Args& m, const Rows16& w, R
     for (int c = c_lo, par = 0;; c += stride, par ^= 1) {
       const int ta = live_lo(c), te = live_hi(c);
       const bool more = c + stride < c_end;  // uniform
-      load_v(c);
+      load_v(c, 0);
+      if constexpr (MAXE > 1) load_v(c, 1);
       if (more) ent = pager.entry_at(32 * (c + stride) + (lane & 31));
       auto next_k = [&]() __attribute__((always_inline)) {
         if (more) {
@@ -487,6 +486,7 @@ __device__ __forceinline__ void rows16_body(const Mx4Args& m, const Rows16& w, R
           mx[e] = fmaxf(fmaxf(mx[e], fmaxf(sc[u][0][e], sc[u][1][e])), fmaxf(sc[u][2][e], sc[u][3][e]));
       }
       if constexpr (MAXE > 1) next_k();
+      else load_v(c, 1);
 
       // the chunk's row maxima: the row's 16 lanes, then the waves
       float(&rm)[4][QROWS] = lds.red_m[par];
@@ -584,8 +584,6 @@ __device__ __forceinline__ void rows16_body(const Mx4Args& m, const Rows16& w, R
         }
       }
 
-      if constexpr (MAXE == 1) next_k();
-
       // the waves' partial sums to LDS, rows of D, the 16-element group x of row p
       // at x ^ (p % 4): lane (kg, i16) holds elements 16 b + i16 of its rows
 #pragma unroll
@@ -632,6 +630,7 @@ __device__ __forceinline__ void rows16_body(const Mx4Args& m, const Rows16& w, R
       // (the next chunk's first barrier stands between these reads and the
       // next writes of the stages and of red_d)
       if (!more) break;
+      if constexpr (MAXE == 1) next_k();
     }
   }
 
