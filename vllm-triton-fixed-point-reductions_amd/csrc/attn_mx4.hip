@@ -20,7 +20,22 @@ struct Planned {
   WsLayout ws;
 };
 
-// Split policy: see the constants.
+// Split policy (bf16, 32 query heads over 8 kv heads of size 128; a chunk is
+// 512 keys).
+// 16-row workgroups split when there are chunks to hand out and the launch is
+// small or its lengths may differ: up to 256 workgroups from two chunks on
+// (16 requests of 2000 keys 20 us, unsplit 25; 4 of 1000 11.8 against 13.6),
+// up to 1024 from four (64 requests of 250 .. 2000 keys 37 us, unsplit 43; all
+// of 2000 56 against 53.5), up to 2048 beyond four (256 requests of
+// 1000 .. 8000 keys 427 us, unsplit 452; all of 8000 758 against 741).  About
+// 6144 workgroups, eight rounds of the card, even the lengths out (64 requests
+// of 16000 keys: 12 splits 381 us, 8 400, 32 388); a request alone has its
+// records read by one workgroup per row, which ends the gain at 128 (64000
+// keys 40.9 us, 64 splits 42.3; over one kv head 18.0 against 22.5).
+// 64-row workgroups split while fewer than two fall to a CU, and up to that:
+// 512 new tokens over 4096 keys 112 us with 2 splits, 145 unsplit, 117 with 8;
+// 128 over 4096 39 us with 8, 144 unsplit; with 512 workgroups 4 x 256 over
+// 2048 95 us unsplit, 119 with 2.
 Planned plan_mx4(int num_requests, int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim, int page_size,
                  int max_query_len, int max_blocks, int window, int int_bits, int requested) {
   Planned r;
@@ -38,10 +53,9 @@ Planned plan_mx4(int num_requests, int64_t num_tokens, int num_heads, int num_kv
     s16 = s64 = std::min<int64_t>({int64_t(requested), slots, kMaxGridZ});
   } else {
     const bool only_long = r.p.rows64 && num_tokens == int64_t(num_requests) * max_query_len;
-    if (chunks > 4 && wgs16 <= 8 * 256 && !only_long) {
-      s16 = std::min<int64_t>(chunks, 64);
-    }
-    if (r.p.rows64 && chunks > 4 && wgs64 < 512) s64 = std::min(cdiv(2048, wgs64), chunks);
+    const int64_t most = chunks < 4 ? 256 : chunks == 4 ? 1024 : 2048;
+    if (wgs16 <= most && !only_long) s16 = std::min(chunks, std::clamp<int64_t>(6144 / wgs16, 8, 128));
+    if (r.p.rows64 && wgs64 < 512) s64 = std::min(cdiv(512, wgs64), chunks);
   }
   auto layout = [&](int64_t rows) { return ws_layout(rows, num_heads, head_dim, int_bits, true, slots); };
   if (s64 > 1 || (s16 > 1 && !r.p.rows64)) {
