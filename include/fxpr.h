@@ -473,7 +473,7 @@ int fxpr_unified_attention_mx4(
 
 /* Workspace bytes fxpr_unified_attention_mx4 needs for this launch (0 = none:
  * also for arguments it rejects). plan: NULL or 4 ints that receive whether
- * requests of 48 query rows per kv head or more run in 64-row workgroups, the
+ * requests of 48 query rows per kv head or more run in the prompts' workgroups, the
  * key splits of those and of the 16-row workgroups, and the tokens per request
  * that have records (0: every token). */
 int64_t fxpr_attention_mx4_plan(int num_requests, int64_t num_tokens,

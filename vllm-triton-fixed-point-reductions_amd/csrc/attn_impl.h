@@ -1704,16 +1704,16 @@ template <int OFF> __device__ __forceinline__ void lds_read_b128_off(unsigned ad
 // tokens and not requests x the longest one (which starts mostly workgroups
 // that exit at once when decode steps share the batch). Wave-uniform; -1 if b
 // belongs to no request.
-__device__ __forceinline__ int flat_block(const AttnArgs& a, int b, int& tile) {
+__device__ __forceinline__ int flat_block(const AttnArgs& a, int b, int& tile, int shift = 6) {
   const int lane = threadIdx.x & 63;
   int owned = 0;  // requests whose first block is at or before b
   for (int r0 = 0; r0 < a.num_requests; r0 += 64) {
     const int r = min(r0 + lane, a.num_requests - 1);
-    const int64_t start = ((int64_t(a.qsl[r]) * a.group) >> 6) + r;
+    const int64_t start = ((int64_t(a.qsl[r]) * a.group) >> shift) + r;
     owned += __builtin_popcountll(__builtin_amdgcn_ballot_w64(r0 + lane < a.num_requests && start <= b));
   }
   const int r = owned - 1;
-  if (r >= 0) tile = b - int(((int64_t(a.qsl[r]) * a.group) >> 6) + r);
+  if (r >= 0) tile = b - int(((int64_t(a.qsl[r]) * a.group) >> shift) + r);
   return r;
 }
 

@@ -32,38 +32,39 @@ struct Planned {
 // of 16000 keys: 12 splits 381 us, 8 400, 32 388); a request alone has its
 // records read by one workgroup per row, which ends the gain at 128 (64000
 // keys 40.9 us, 64 splits 42.3; over one kv head 18.0 against 22.5).
-// 64-row workgroups split while fewer than two fall to a CU, and up to that:
-// 512 new tokens over 4096 keys 112 us with 2 splits, 145 unsplit, 117 with 8;
-// 128 over 4096 39 us with 8, 144 unsplit; with 512 workgroups 4 x 256 over
-// 2048 95 us unsplit, 119 with 2.
+// The prompts' workgroups (128 rows) split while fewer than two fall to a CU,
+// and up to that: 512 new tokens over 4096 keys 94 us with 4 splits, 205 unsplit,
+// 97 with 8; 128 over 16000 97 us with 16, 788 unsplit; 4 x 256 over 4096 180 us
+// with 2, 209 unsplit; with 512 workgroups, 2048 over 4096, 249 us unsplit, 292
+// with 2.
 Planned plan_mx4(int num_requests, int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim, int page_size,
                  int max_query_len, int max_blocks, int window, int int_bits, int requested) {
   Planned r;
   const int group = num_heads / num_kv_heads;
   const int64_t slots = std::max<int64_t>(chunk_slots(max_blocks, page_size), 1);
   const int64_t max_rows = int64_t(max_query_len > 1 ? max_query_len : 1) * group;
-  r.p.rows64 = max_rows >= kPrefillRows;
-  const int64_t qtiles = std::min<int64_t>(cdiv(max_rows, QROWS), r.p.rows64 ? kShortTiles : int64_t(1) << 40);
+  r.p.prompt = max_rows >= kPrefillRows;
+  const int64_t qtiles = std::min<int64_t>(cdiv(max_rows, QROWS), r.p.prompt ? kShortTiles : int64_t(1) << 40);
   const int64_t wgs16 = int64_t(num_requests) * num_kv_heads * qtiles;
-  const int64_t wgs64 = std::max<int64_t>(cdiv(num_tokens * num_heads, PQROWS), 1);
+  const int64_t wgsp = std::max<int64_t>(cdiv(num_tokens * num_heads, row_sets(int_bits, head_dim) * PQROWS), 1);
   // chunks that a row's keys can touch
   const int64_t chunks = window > 0 ? std::min(slots, cdiv(int64_t(window) + max_query_len, TILE * CT) + 1) : slots;
-  int64_t s16 = 1, s64 = 1;
+  int64_t s16 = 1, sp = 1;
   if (requested >= 1) {
-    s16 = s64 = std::min<int64_t>({int64_t(requested), slots, kMaxGridZ});
+    s16 = sp = std::min<int64_t>({int64_t(requested), slots, kMaxGridZ});
   } else {
-    const bool only_long = r.p.rows64 && num_tokens == int64_t(num_requests) * max_query_len;
+    const bool only_long = r.p.prompt && num_tokens == int64_t(num_requests) * max_query_len;
     const int64_t most = chunks < 4 ? 256 : chunks == 4 ? 1024 : 2048;
     if (wgs16 <= most && !only_long) s16 = std::min(chunks, std::clamp<int64_t>(6144 / wgs16, 8, 128));
-    if (r.p.rows64 && wgs64 < 512) s64 = std::min(cdiv(512, wgs64), chunks);
+    if (r.p.prompt && wgsp < 512) sp = std::min(cdiv(512, wgsp), chunks);
   }
   auto layout = [&](int64_t rows) { return ws_layout(rows, num_heads, head_dim, int_bits, true, slots); };
-  if (s64 > 1 || (s16 > 1 && !r.p.rows64)) {
+  if (sp > 1 || (s16 > 1 && !r.p.prompt)) {
     r.ws = layout(num_tokens);
     if (r.ws.total > kMx4WsMax) {
       r.ws = WsLayout{};
-      if (!r.p.rows64 || requested >= 1) s16 = 1;
-      s64 = 1;
+      if (!r.p.prompt || requested >= 1) s16 = 1;
+      sp = 1;
     }
   }
   if (r.ws.total == 0 && s16 > 1) {
@@ -78,7 +79,7 @@ Planned plan_mx4(int num_requests, int64_t num_tokens, int num_heads, int num_kv
     }
   }
   r.p.splits = int(s16);
-  r.p.pq_splits = int(s64);
+  r.p.pq_splits = int(sp);
   return r;
 }
 
@@ -98,7 +99,7 @@ extern "C" int64_t fxpr_attention_mx4_plan(int num_requests, int64_t num_tokens,
   const Planned p = plan_mx4(num_requests, num_tokens, num_heads, num_kv_heads, head_dim, page_size, max_query_len,
                              max_blocks_per_seq, std::max(window_size, 0), int_bits, num_kv_splits);
   if (plan) {
-    plan[0] = p.p.rows64 ? 1 : 0;
+    plan[0] = p.p.prompt ? 1 : 0;
     plan[1] = p.p.pq_splits;
     plan[2] = p.p.splits;
     plan[3] = p.p.tok_cap;

@@ -16,7 +16,7 @@
 //   attn_mx4_rows16_kernel  16 query rows a workgroup (decode, short prompts).
 //     Bound by the cache's bytes, so its four waves take different key tiles of
 //     a chunk and share nothing but the chunk's maxima and integer sums.
-//   attn_mx4_rows64_kernel  64 query rows (prompts). Bound by vector
+//   attn_mx4_prompt_kernel  128 query rows, or 64 (prompts). Bound by vector
 //     arithmetic, so a key tile is unpacked once for the four waves.
 #pragma once
 
@@ -86,11 +86,19 @@ __device__ __forceinline__ int turned(const Mx4Args& m, int x, int pass) {
 constexpr float kRoundF = 12582912.0f;
 constexpr uint32_t kRound = 0x4B400000u;
 
+// Sets of 64 query rows of a prompt's workgroup (16 a wave): two where their
+// sums fit a wave's registers (but for the folded ones, which a chunk's end
+// alone needs and takes from scratch). Two sets take a key tile's unpacking, LDS
+// reads and barrier once: four prompts of up to 2048 tokens 208 us, one set 253
+// (235 with a third workgroup per CU); 8 x 512 new tokens over 16000 keys 2.26 ms
+// against 2.70.
+constexpr int row_sets(int bits, int head_dim) { return bits != 64 && head_dim <= 128 ? 2 : 1; }
+
 // Host plan of a launch.
 struct Mx4Plan {
   int splits = 1;            // key splits of the 16-row workgroups (every splits-th chunk)
-  int pq_splits = 1;         // of the 64-row workgroups (chunks dealt evenly)
-  bool rows64 = false;       // requests of kPrefillRows rows or more in 64-row workgroups
+  int pq_splits = 1;         // of the prompts' workgroups (chunks dealt evenly)
+  bool prompt = false;       // requests of kPrefillRows rows or more in the prompts' workgroups
   int tok_cap = 0;           // AttnArgs::tok_cap
 };
 
@@ -249,7 +257,7 @@ template <class A> __device__ __forceinline__ Pager make_pager(const A& a, int r
 // MFMA's rows), row p as MFMA row 4 (p % 4) + p / 4: lane group kg then has rows
 // kg, kg + 4, .. in its result registers e = 0, 1, .., and with 4 rows only
 // e = 0 holds any. The softmax and the sums run over NE of the 4 registers (the
-// transposed layout of the 64-row kernel has no register to leave out: 102 us
+// transposed layout of the prompts' kernel has no register to leave out: 102 us
 // for 64 requests up to 8192 keys, where the weights cross LDS here).
 //
 // FAST (the same bits): no softcap or ALiBi and a positive scale, so a score is
@@ -674,7 +682,7 @@ __global__ __launch_bounds__(kThreads, (rows16_wgs<BITS, D, MAXE>())) void attn_
   const int rows_total = w.q_len * a.group;
   w.row0 = blockIdx.y * (MAXE == 4 ? QROWS : 4 * MAXE);
   if (w.row0 >= rows_total) return;                        // uniform
-  if (a.pq_rows > 0 && rows_total >= a.pq_rows) return;  // attn_mx4_rows64_kernel's request
+  if (a.pq_rows > 0 && rows_total >= a.pq_rows) return;  // attn_mx4_prompt_kernel's request
   if (a.window > 0) {
     const int i_min = int(quotient(uint32_t(w.row0), m.by_group));
     const int c = max(0, w.ctx + i_min - a.window + 1) / (TILE * CT) + (SPLIT ? int(blockIdx.z) : 0);
@@ -690,18 +698,34 @@ __global__ __launch_bounds__(kThreads, (rows16_wgs<BITS, D, MAXE>())) void attn_
 }
 
 // ---------------------------------------------------------------------------
-// 64 query rows, 16 a wave. A chunk's K tiles are read twice, for the row
-// maxima (two tiles a step) and, with the V tiles, for the weights, as in
-// attn_impl.h's prefill kernels. A step has two tiles in LDS (K K or K V), the
-// next step's in registers, packed, and those of the step after on their way;
-// a step's tiles are unpacked into the other half of the LDS between the MFMAs
-// of the step before. Steps alternate between two halves of the code, so LDS
-// addresses and registers are fixed (an odd step is padded with one that only
-// moves data). The table entries of a chunk are one vector load, its granules'
-// offsets a lane each (scalar loads in the loop are waited for together with
-// the LDS reads: 397 us for four prompts of up to 2048 tokens with them and
-// one step's prefetch).
+// Prompts: RS sets of 16 query rows a wave. A chunk's K tiles are read twice, for the row
+// maxima and, alternating with the V tiles, for the weights, as in attn_impl.h's
+// prefill kernels. A step is one tile: it lies in one of two LDS tiles while the
+// next one is unpacked into the other between the MFMAs; the two after that are
+// on their way in registers, packed. Steps alternate between two halves of the
+// code, so LDS addresses and registers are fixed (an odd number of first steps is
+// padded with one that only moves data). The table entries of a chunk are one
+// vector load, its granules' offsets a lane each, kept for two chunks at once: a
+// step's addresses are scalar (scalar loads in the loop are waited for together
+// with the LDS reads; moving the lanes on at a chunk's end within the loop cost
+// 20 moves a step and a wait for the prefetch).
 //
+// Four prompts of up to 2048 tokens, 32 heads over 8 of 128, bf16: 208 us, 398
+// TFLOP/s of the products that the formula has (the K products are made twice).
+// Vector instructions are issued in 60 of 100 cycles, MFMAs run in 27, the LDS
+// works in 30; two waves per SIMD leave the rest.
+//
+// LDS rows are padded: a row's 16-byte chunk x is at row * PITCH + (row / 8) *
+// OCT + 16 x, so that every read is a constant away from one address. With 64
+// bytes of padding four consecutive rows take different quarters of the banks;
+// OCT keeps apart the rows 8 k + .. of a K fragment read (16) and of half a
+// wave's transposing V read (32).
+template <int D> struct PromptLds {
+  static constexpr int PITCH = Lds<D>::ROWB + 64;
+  static constexpr int KOCT = 16, VOCT = 32;
+  static constexpr int TILEB = TILE * PITCH + 8 * VOCT;
+};
+
 // SPLIT: the chunks of a row tile are dealt evenly to pq_splits workgroups; the
 // first folds its chunks and leaves the folded state as one record, the others
 // a record per chunk.
@@ -709,15 +733,15 @@ __global__ __launch_bounds__(kThreads, (rows16_wgs<BITS, D, MAXE>())) void attn_
 // FAST as in the 16-row kernel, and over a softcap too (CAP): the softcap is
 // monotone, so the chunk maximum is the capped maximum of the raw scores, and
 // only phase 1 computes a score's tanh.
-template <int DT, int BITS, int D, bool SPLIT, bool FAST, bool CAP>
-__global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void attn_mx4_rows64_kernel(Mx4Args m) {
+template <int DT, int BITS, int D, bool SPLIT, bool FAST, bool CAP, int RS>
+__global__ __launch_bounds__(kPThreads, D == 256 ? 1 : 2) void attn_mx4_prompt_kernel(Mx4Args m) {
   const AttnArgs& a = m.a;
   using TR = Traits<DT>;
   using T = typename TR::T;
   using AccT = typename AccOf<BITS>::T;
-  using L = Lds<D>;
-  constexpr int QS = D / 32, DBLK = D / 16;
-  extern __shared__ __align__(16) unsigned char lds[];  // [2][2] tiles
+  using RL = PromptLds<D>;
+  constexpr int QS = D / 32, DBLK = D / 16, ROWS = RS * PQROWS;
+  extern __shared__ __align__(16) unsigned char lds[];  // [2] tiles
 
   const int tid = threadIdx.x, lane = tid & 63, kg = lane >> 4, i16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -726,7 +750,7 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
   int rtile = int(gridDim.y) - 1 - int(blockIdx.y);  // the longest row tiles first
   if (a.pq_blocks == 0) r = turned(m, r, int(blockIdx.z * gridDim.y + blockIdx.y));
   if (a.pq_blocks > 0) {
-    r = __builtin_amdgcn_readfirstlane(flat_block(a, a.pq_blocks - 1 - r, rtile));
+    r = __builtin_amdgcn_readfirstlane(flat_block(a, a.pq_blocks - 1 - r, rtile, RS == 2 ? 7 : 6));
     rtile = __builtin_amdgcn_readfirstlane(rtile);
     if (r < 0 || rtile < 0) return;  // uniform
   }
@@ -735,12 +759,12 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
   const int seq_len = ((ConstI32)a.seq_lens)[r];
   const int ctx = seq_len - q_len;
   const int rows_total = q_len * a.group;
-  const int row0 = rtile * PQROWS;
+  const int row0 = rtile * ROWS;
   if (row0 >= rows_total || rows_total < a.pq_rows) return;  // uniform
-  const int wrow0 = row0 + 16 * wave;
+  const int wrow0 = row0 + 16 * RS * wave;
 
   const int i_min = int(quotient(uint32_t(row0), m.by_group));
-  const int i_max = int(quotient(uint32_t(min(rows_total - 1, row0 + PQROWS - 1)), m.by_group));
+  const int i_max = int(quotient(uint32_t(min(rows_total - 1, row0 + ROWS - 1)), m.by_group));
   const int hi = a.causal ? min(seq_len, ctx + i_max + 1) : seq_len;
   const int lo = a.window > 0 ? max(0, ctx + i_min - a.window + 1) : 0;
   const int t_lo = lo / TILE;
@@ -761,44 +785,42 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
   auto live_hi = [&](int c) { return min(c * CT + CT, t_hi); };
 
   // The stream of steps. Chunk c with n live tiles from ta has steps0(n) steps of
-  // phase 0 (K tiles 2 k, 2 k + 1) and steps1(n) of phase 1 (K and V of tile k),
-  // both even; tiles past the last are the last again.
-  auto steps0 = [](int n) { return 2 * ((n + 3) >> 2); };
-  auto steps1 = [](int n) { return 2 * ((n + 1) >> 1); };
-  // The staging cursor: the next step to load. A lane holds the byte offsets and
-  // limits (Pager) of granule `lane` of its chunk (32 granules).
-  int fc = c_lo, fphase = 0, fk = 0, fta = 0, fn = 1;
+  // phase 0 (K tile k, past the last the last again) and 2 n of phase 1 (K, V of
+  // tile k / 2).
+  auto steps0 = [](int n) { return 2 * ((n + 1) >> 1); };
+  // Byte offsets and limits (Pager) of the granules of two chunks, a lane each:
+  // granule l of chunk c in lane 32 (c % 2) + l.
   uint32_t oc_lo = 0, oc_hi = 0, os_lo = 0, os_hi = 0, lim_c = 0, lim_s = 0;
-  int ent = 0;  // the table entry of the lane's granule of chunk fc, then of chunk fc + 1
-  auto load_entry = [&](int c) { ent = a.bt[int64_t(r) * a.sbt + min((16 * pager.granule(32 * c + (lane & 31))) >> pager.ps_shift,
-                                                                    pager.max_blocks - 1)]; };
-  auto open_chunk = [&]() __attribute__((always_inline)) {
-    fta = live_lo(fc);
-    fn = live_hi(fc) - fta;
-    const int gq = pager.granule(32 * fc + (lane & 31));
+  auto open_chunk = [&](int c, int ent, bool mine) __attribute__((always_inline)) {
+    const int gq = pager.granule(32 * c + (lane & 31));
     const uint64_t oc = pager.offset(gq, ent, m.c_blk, m.c_slot, ch), os = pager.offset(gq, ent, m.s_blk, m.s_slot, sh);
-    oc_lo = uint32_t(oc);
-    oc_hi = uint32_t(oc >> 32);
-    os_lo = uint32_t(os);
-    os_hi = uint32_t(os >> 32);
-    lim_c = pager.limit(gq, m.c_slot) + 3 * (D / 8);
-    lim_s = pager.limit(gq, m.s_slot);
-    if (fc + 1 < c_hi) load_entry(fc + 1);
+    oc_lo = mine ? uint32_t(oc) : oc_lo;
+    oc_hi = mine ? uint32_t(oc >> 32) : oc_hi;
+    os_lo = mine ? uint32_t(os) : os_lo;
+    os_hi = mine ? uint32_t(os >> 32) : os_hi;
+    lim_c = mine ? pager.limit(gq, m.c_slot) + 3 * (D / 8) : lim_c;
+    lim_s = mine ? pager.limit(gq, m.s_slot) : lim_s;
+  };
+  auto entry_of = [&](int c) { return pager.entry_at(pager.granule(32 * c + (lane & 31))); };
+  int ent = 0;  // the table entry of the lane's granule of the chunk after the open ones
+  // The staging cursor: the next step to load, and the lane of its chunk's first
+  // live granule of the wave.
+  int fc = c_lo, fphase = 0, fk = 0, fn = 1, fl = 0;
+  auto enter = [&]() __attribute__((always_inline)) {
+    const int ta = live_lo(fc);
+    fn = live_hi(fc) - ta;
+    fl = 32 * (fc & 1) + 4 * (ta - CT * fc) + wave;
   };
   auto advance = [&]() __attribute__((always_inline)) {
     ++fk;
-    if (fphase == 0) {
-      if (fk >= steps0(fn)) {
-        fphase = 1;
-        fk = 0;
-      }
-    } else if (fk >= steps1(fn)) {
-      if (fc + 1 < c_hi) {
-        ++fc;
-        fphase = fk = 0;
-        open_chunk();
+    if (fk >= (fphase ? 2 * fn : steps0(fn))) {
+      if (fphase && fc + 1 >= c_hi) {
+        --fk;  // past the end: the last tile again
       } else {
-        --fk;  // past the end: the last step again
+        fk = 0;
+        fc += fphase;
+        fphase ^= 1;
+        enter();
       }
     }
   };
@@ -813,7 +835,7 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
   const uint32_t c_off = uint32_t(lane >> 2) * m.c_slot + (lane & 3) * (D / 8), s_off = uint32_t(lane >> 2) * m.s_slot;
   auto at_lane = [](uint32_t x, int l) { return uint32_t(__builtin_amdgcn_readlane(int(x), l)); };
   auto fetch = [&](const uint8_t* codes, const uint8_t* scales, int k) __attribute__((always_inline)) {
-    const int l = 4 * (fta + min(k, fn - 1) - CT * fc) + wave;  // the granule in its chunk
+    const int l = fl + 4 * min(k, fn - 1);
     const uint8_t* cp = codes + ((uint64_t(at_lane(oc_hi, l)) << 32) | at_lane(oc_lo, l));
     const uint8_t* sp = scales + ((uint64_t(at_lane(os_hi, l)) << 32) | at_lane(os_lo, l));
     Staged x;
@@ -821,75 +843,78 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
     x.s = load_scales<D>(sp + min(s_off, at_lane(lim_s, l)));
     return x;
   };
-  Staged r0[2], r1[2];  // by the step's parity
-  auto fetch0 = [&](Staged& x) __attribute__((always_inline)) { x = fetch(m.kc, m.ks, fphase ? fk : 2 * fk); };
-  auto fetch1 = [&](Staged& x) __attribute__((always_inline)) {
-    x = fetch(fphase ? m.vc : m.kc, fphase ? m.vs : m.ks, fphase ? fk : 2 * fk + 1);
+  Staged st[2];  // by the step's parity
+  auto refill = [&](Staged& x) __attribute__((always_inline)) {
+    const bool v = (fphase & fk) != 0;
+    x = fetch(v ? m.vc : m.kc, v ? m.vs : m.ks, fk >> fphase);
+    advance();
   };
-  unsigned kwr[QS], vwr[QS];
-#pragma unroll
-  for (int j = 0; j < QS; ++j) {
-    kwr[j] = srow * L::ROWB + (((4 * j + (lane & 3)) ^ L::kswz(srow)) << 4);
-    vwr[j] = srow * L::ROWB + (((4 * j + (lane & 3)) ^ L::vswz(srow)) << 4);
-  }
-  // unit j of a staged tile into LDS tile `tile` (of four)
-  auto put = [&](const Staged& x, int tile, const unsigned (&at)[QS], int j) __attribute__((always_inline)) {
-    lds_store16(lds + tile * L::TILEB + at[j], mx4::unpack8<DT>(x.u.w[j], mx4::scale_of<DT>(x.s.w[j / 4], j % 4)));
+  const unsigned wr_row = srow * RL::PITCH + (lane & 3) * 16;
+  const unsigned k_wr = wr_row + (srow >> 3) * RL::KOCT, v_wr = wr_row + (srow >> 3) * RL::VOCT;
+  // unit j of a staged tile into LDS at `at`
+  auto put = [&](const Staged& x, unsigned at, int j) __attribute__((always_inline)) {
+    lds_store16(lds + at + 64 * j, mx4::unpack8<DT>(x.u.w[j], mx4::scale_of<DT>(x.s.w[j / 4], j % 4)));
   };
   if (c_lo < c_hi) {
-    load_entry(fc);
-    open_chunk();
-    fetch0(r0[0]);
-    fetch1(r1[0]);
-    advance();
-    fetch0(r0[1]);
-    fetch1(r1[1]);
-    advance();
+    const int c = c_lo + ((lane >> 5) ^ (c_lo & 1));
+    open_chunk(c, entry_of(c), true);
+    ent = entry_of(c_lo + 2);
+    enter();
+    refill(st[0]);
+    refill(st[1]);
   }
 
-  // The lane's query row.
-  const RowInfo me = row_at(m, g, q_start, q_len, ctx, seq_len, wrow0 + i16);
-  u32x4 qf[QS];
-  {
+  // The lane's query rows, one of each set of 16.
+  u32x4 qf[RS][QS];
+  int ks[RS], ke[RS], qp[RS];
+  float slope[RS];
+#pragma unroll
+  for (int u = 0; u < RS; ++u) {
+    const RowInfo me = row_at(m, g, q_start, q_len, ctx, seq_len, wrow0 + 16 * u + i16);
     const T* qbase = static_cast<const T*>(a.q) + me.token * a.sq_t + int64_t(me.head) * a.sq_h;
 #pragma unroll
     for (int j = 0; j < QS; ++j)
-      qf[j] = me.valid ? *reinterpret_cast<const u32x4*>(qbase + 32 * j + 8 * kg) : u32x4{0u, 0u, 0u, 0u};
+      qf[u][j] = me.valid ? *reinterpret_cast<const u32x4*>(qbase + 32 * j + 8 * kg) : u32x4{0u, 0u, 0u, 0u};
+    ks[u] = me.valid ? me.kstart : 0x7fffffff;
+    ke[u] = me.valid ? me.kend : 0;
+    qp[u] = me.qpos;
+    slope[u] = !FAST && a.alibi ? a.alibi[me.head] : 0.0f;
   }
-  const int ks = me.valid ? me.kstart : 0x7fffffff;
-  const int ke = me.valid ? me.kend : 0;
-  const int qp = me.qpos;
-  const float slope = !FAST && a.alibi ? a.alibi[me.head] : 0.0f;
+  // (worked out again where it is stored: fewer registers over the loop)
+  auto row_of = [&](int u) __attribute__((always_inline)) {
+    int row = wrow0 + 16 * u;
+    asm volatile("" : "+s"(row));
+    return row_at(m, g, q_start, q_len, ctx, seq_len, row + i16);
+  };
   auto tile_whole = [&](int t) -> bool {
-    return __builtin_amdgcn_ballot_w64(!(ks <= t * TILE && t * TILE + TILE <= ke)) == 0;
+    bool part = false;
+#pragma unroll
+    for (int u = 0; u < RS; ++u) part |= !(ks[u] <= t * TILE && t * TILE + TILE <= ke[u]);
+    return __builtin_amdgcn_ballot_w64(part) == 0;
   };
 
-  // LDS offsets of the score MFMAs' K rows pi(i16) (step s: + 32 rows, which
-  // the swizzle ignores) and of the transposing V reads, as in attn_impl.h.
-  unsigned koff[2][QS];
+  // LDS addresses: the score MFMAs' K rows 8 (i16 / 4) + i16 % 4 (h: 4 rows on, s:
+  // 32 rows on), chunks 4 j + kg; the transposing V reads, rows 8 kg + i16 / 4,
+  // columns 4 (i16 % 4) of d block 0 (d block b: 32 b on).
+  const unsigned k_rd = (8 * (i16 >> 2) + (i16 & 3)) * RL::PITCH + (i16 >> 2) * RL::KOCT + kg * 16;
+  const unsigned v_rd = (8 * kg + (i16 >> 2)) * RL::PITCH + kg * RL::VOCT + (i16 & 3) * 8;
+  constexpr unsigned kStepK = 32 * RL::PITCH + 4 * RL::KOCT, kStepV = 32 * RL::PITCH + 4 * RL::VOCT;
+
+  float Mr[RS];
+  AccT Dr[RS];
+  AccT Wr[RS][DBLK][4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int u = 0; u < RS; ++u) {
+    Mr[u] = -__builtin_inff();
+    Dr[u] = 0;
 #pragma unroll
-    for (int j = 0; j < QS; ++j) {
-      const int rr = 8 * (i16 >> 2) + 4 * h + (i16 & 3);
-      koff[h][j] = rr * L::ROWB + (((4 * j + kg) ^ L::kswz(rr)) << 4);
-    }
-  unsigned vrd[2];
+    for (int b = 0; b < DBLK; ++b)
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int rr = 8 * kg + (i16 >> 2) + 4 * h;
-    vrd[h] = rr * L::ROWB + ((((i16 & 3) >> 1) ^ L::vswz(rr)) << 4) + (i16 & 1) * 8;
+      for (int e = 0; e < 4; ++e) Wr[u][b][e] = 0;
   }
 
-  float Mr = -__builtin_inff();
-  AccT Dr = 0;
-  AccT Wr[DBLK][4];
-#pragma unroll
-  for (int b = 0; b < DBLK; ++b)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) Wr[b][e] = 0;
-
-  auto store_record = [&](int c, float mc, AccT den, const AccT (&w)[DBLK][4]) __attribute__((always_inline)) {
+  auto store_record = [&](int u, int c, float mc, AccT den, const AccT (&w)[DBLK][4]) __attribute__((always_inline)) {
+    const RowInfo me = row_of(u);
     if (!me.valid) return;
     const int64_t slot = (me.token * a.num_heads + me.head) * a.chunk_slots + c;
     if (kg == 0) {
@@ -909,27 +934,32 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
     auto issue = [&](auto qc) __attribute__((always_inline)) {
       constexpr int q = decltype(qc)::value;
 #pragma unroll
-      for (int j = 0; j < QS; ++j) kf[q & 1][j] = lds_load16(tile + (q >> 1) * 32 * L::ROWB + koff[q & 1][j]);
+      for (int j = 0; j < QS; ++j) kf[q & 1][j] = lds_load16(tile + k_rd + ((q >> 1) * kStepK + (q & 1) * 4 * RL::PITCH + 64 * j));
     };
     issue(std::integral_constant<int, 0>{});
-    f32x4 accs[2];
+    f32x4 accs[2][RS];
     static_for<4>([&](auto qc) __attribute__((always_inline)) {
       constexpr int q = decltype(qc)::value;
       if constexpr (q + 1 < 4) issue(std::integral_constant<int, q + 1>{});
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < QS; ++j) acc = TR::mma(kf[q & 1][j], qf[j], acc);
-      accs[q & 1] = acc;
+      for (int u = 0; u < RS; ++u) accs[q & 1][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < QS; ++j)
+#pragma unroll
+        for (int u = 0; u < RS; ++u) accs[q & 1][u] = TR::mma(kf[q & 1][j], qf[u][j], accs[q & 1][u]);
       side(qc);
-      if constexpr (q > 0) fn(std::integral_constant<int, q - 1>{}, accs[(q - 1) & 1]);
+      if constexpr (q > 0)
+#pragma unroll
+        for (int u = 0; u < RS; ++u) fn(std::integral_constant<int, q - 1>{}, u, accs[(q - 1) & 1][u]);
       __builtin_amdgcn_sched_barrier(0);
     });
-    fn(std::integral_constant<int, 3>{}, accs[1]);
+#pragma unroll
+    for (int u = 0; u < RS; ++u) fn(std::integral_constant<int, 3>{}, u, accs[1][u]);
   };
   auto capped = [&](float x) { return softcapped(x, a.softcap_log2); };
   // Scores of chain q for the lane's row and keys t * TILE + 32 (q / 2) + 8 kg +
   // 4 (q % 2) + e. (RAW: before the softcap; the mask is -inf, a score is not.)
-  auto chain_scores = [&](const f32x4& acc, int t, int q, bool whole, auto raw_tag, float (&sc)[4])
+  auto chain_scores = [&](const f32x4& acc, int t, int u, int q, bool whole, auto raw_tag, float (&sc)[4])
                           __attribute__((always_inline)) {
     constexpr bool RAW = decltype(raw_tag)::value;
     const int key0 = t * TILE + 32 * (q >> 1) + 8 * kg + 4 * (q & 1);
@@ -938,268 +968,275 @@ __global__ __launch_bounds__(kPThreads, D == 256 || BITS == 64 ? 1 : 2) void att
       float x = __fmul_rn(acc[e], a.scale_log2);
       if constexpr (!FAST) {
         if (a.softcap_log2 > 0.0f) x = capped(x);
-        if (a.alibi) x = x + slope * static_cast<float>(key0 + e - qp);
+        if (a.alibi) x = x + slope[u] * static_cast<float>(key0 + e - qp[u]);
       } else if constexpr (CAP) {
         x = RAW ? fmaxf(x, -kFltMax) : capped(x);
       }
-      sc[e] = (whole || (key0 + e >= ks && key0 + e < ke)) ? x : -__builtin_inff();
+      sc[e] = (whole || (key0 + e >= ks[u] && key0 + e < ke[u])) ? x : -__builtin_inff();
     }
   };
 
   if (c_lo < c_hi) {
-    // the first step's tiles (K K) to LDS; two more steps on their way
+    // the first step's tile to LDS; two more on their way
 #pragma unroll
-    for (int j = 0; j < QS; ++j) put(r0[0], 0, kwr, j);
-#pragma unroll
-    for (int j = 0; j < QS; ++j) put(r1[0], 1, kwr, j);
-    fetch0(r0[0]);
-    fetch1(r1[0]);
-    advance();
-    // a part of the units of the next step's first and second tile, beside the
-    // MFMAs of this one (parity P); VNEXT: its second tile is a V tile
+    for (int j = 0; j < QS; ++j) put(st[0], k_wr, j);
+    refill(st[0]);
+    // part q (of four) of unpacking the tile of the step after one of parity P
     constexpr int UPP = QS >= 4 ? QS / 4 : 1;
-    auto put0 = [&](auto pc, auto qc) __attribute__((always_inline)) {
+    auto put_part = [&](auto pc, unsigned at, auto qc) __attribute__((always_inline)) {
       constexpr int P = decltype(pc)::value, q = decltype(qc)::value;
 #pragma unroll
-      for (int j = q * UPP; j < (q + 1) * UPP && j < QS; ++j) put(r0[P ^ 1], 2 * (P ^ 1), kwr, j);
-    };
-    auto put1 = [&](auto pc, auto qc, bool vnext) __attribute__((always_inline)) {
-      constexpr int P = decltype(pc)::value, q = decltype(qc)::value;
-#pragma unroll
-      for (int j = q * UPP; j < (q + 1) * UPP && j < QS; ++j) {
-        if constexpr (D == 64) put(r1[P ^ 1], 2 * (P ^ 1) + 1, vnext ? vwr : kwr, j);
-        else put(r1[P ^ 1], 2 * (P ^ 1) + 1, kwr, j);  // (the K swizzle is the V one)
-      }
-    };
-    auto put_all0 = [&](auto pc) __attribute__((always_inline)) { static_for<4>([&](auto qc) { put0(pc, qc); }); };
-    auto put_all1 = [&](auto pc, bool vnext) __attribute__((always_inline)) {
-      static_for<4>([&](auto qc) { put1(pc, qc, vnext); });
-    };
-    auto refill0 = [&](auto pc) __attribute__((always_inline)) { fetch0(r0[decltype(pc)::value ^ 1]); };
-    auto refill1 = [&](auto pc) __attribute__((always_inline)) {
-      fetch1(r1[decltype(pc)::value ^ 1]);
-      advance();
+      for (int j = q * UPP; j < (q + 1) * UPP && j < QS; ++j) put(st[P ^ 1], (P ^ 1) * RL::TILEB + at, j);
     };
 
     for (int c = c_lo; c < c_hi; ++c) {
-      const int ta = live_lo(c), te = live_hi(c), n0 = steps0(te - ta), n1 = steps1(te - ta);
-      float mx = -__builtin_inff(), mraw = -__builtin_inff();
+      const int ta = live_lo(c), te = live_hi(c), n0 = steps0(te - ta);
+      // (the cursor has left chunk c - 1 and is in chunk c: both have four steps or more)
+      if (c > c_lo && c + 1 < c_hi) {
+        open_chunk(c + 1, ent, (lane >> 5) == ((c + 1) & 1));
+        ent = entry_of(c + 2);
+      }
+      float mx[RS], mraw[RS];
+#pragma unroll
+      for (int u = 0; u < RS; ++u) mx[u] = mraw[u] = -__builtin_inff();
       // phase 0: the chunk's row maxima
       auto max_tile = [&](int t, const unsigned char* tile, auto&& side) __attribute__((always_inline)) {
         if (FAST && tile_whole(t)) {
-          scores_of(tile, side, [&](auto, const f32x4& acc) __attribute__((always_inline)) {
-            mraw = fmaxf(fmaxf(mraw, fmaxf(acc[0], acc[1])), fmaxf(acc[2], acc[3]));
+          scores_of(tile, side, [&](auto, int u, const f32x4& acc) __attribute__((always_inline)) {
+            mraw[u] = fmaxf(fmaxf(mraw[u], fmaxf(acc[0], acc[1])), fmaxf(acc[2], acc[3]));
           });
-          if constexpr (CAP) mraw = fmaxf(mraw, -kFltMax);  // keys were seen
+          if constexpr (CAP)  // keys were seen
+#pragma unroll
+            for (int u = 0; u < RS; ++u) mraw[u] = fmaxf(mraw[u], -kFltMax);
         } else {
-          scores_of(tile, side, [&](auto qc, const f32x4& acc) __attribute__((always_inline)) {
+          scores_of(tile, side, [&](auto qc, int u, const f32x4& acc) __attribute__((always_inline)) {
             float sc[4];
-            chain_scores(acc, t, decltype(qc)::value, false, std::true_type{}, sc);
-            mx = fmaxf(fmaxf(mx, fmaxf(sc[0], sc[1])), fmaxf(sc[2], sc[3]));
+            chain_scores(acc, t, u, decltype(qc)::value, false, std::true_type{}, sc);
+            mx[u] = fmaxf(fmaxf(mx[u], fmaxf(sc[0], sc[1])), fmaxf(sc[2], sc[3]));
           });
         }
       };
-      auto step0 = [&](auto pc, int k) __attribute__((always_inline)) {
+      auto step0 = [&](auto pc, int t) __attribute__((always_inline)) {
         constexpr int P = decltype(pc)::value;
-        const int t = ta + 2 * k;
-        const bool vnext = k + 1 >= n0;
         lds_barrier();
-        if (t < te) max_tile(t, lds + 2 * P * L::TILEB, [&](auto qc) { put0(pc, qc); });
-        else put_all0(pc);
-        refill0(pc);
-        if (t + 1 < te) max_tile(t + 1, lds + (2 * P + 1) * L::TILEB, [&](auto qc) { put1(pc, qc, vnext); });
-        else put_all1(pc, vnext);
-        refill1(pc);
+        if (t < te) max_tile(t, lds + P * RL::TILEB, [&](auto qc) { put_part(pc, k_wr, qc); });
+        else static_for<4>([&](auto qc) { put_part(pc, k_wr, qc); });
+        refill(st[P ^ 1]);
       };
       for (int k = 0; k < n0; k += 2) {
-        step0(std::integral_constant<int, 0>{}, k);
-        step0(std::integral_constant<int, 1>{}, k + 1);
+        step0(std::integral_constant<int, 0>{}, ta + k);
+        step0(std::integral_constant<int, 1>{}, ta + k + 1);
       }
-      if constexpr (FAST) {
-        float m1 = __fmul_rn(mraw, a.scale_log2);
-        if constexpr (CAP) m1 = mraw != -__builtin_inff() ? fmaxf(m1, -kFltMax) : m1;
-        mx = fmaxf(mx, m1);
+      float mrow[RS];
+#pragma unroll
+      for (int u = 0; u < RS; ++u) {
+        if constexpr (FAST) {
+          float m1 = __fmul_rn(mraw[u], a.scale_log2);
+          if constexpr (CAP) m1 = mraw[u] != -__builtin_inff() ? fmaxf(m1, -kFltMax) : m1;
+          mx[u] = fmaxf(mx[u], m1);
+        }
+        mx[u] = fmaxf(mx[u], __shfl_xor(mx[u], 16, 64));
+        mx[u] = fmaxf(mx[u], __shfl_xor(mx[u], 32, 64));
+        if constexpr (CAP) mx[u] = mx[u] != -__builtin_inff() ? capped(mx[u]) : mx[u];
+        mrow[u] = mx[u] != -__builtin_inff() ? mx[u] : 0.0f;  // no key: pin to 0
       }
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      if constexpr (CAP) mx = mx != -__builtin_inff() ? capped(mx) : mx;
-      const float mrow = mx != -__builtin_inff() ? mx : 0.0f;  // no key: pin to 0
       // phase 1: weights and weighted V. FAST: the sums carry kRound per added
       // term, taken out at the chunk's end.
-      AccT den = 0;
-      AccT wv[DBLK][4];
+      AccT den[RS];
+      AccT wv[RS][DBLK][4];
 #pragma unroll
-      for (int b = 0; b < DBLK; ++b)
+      for (int u = 0; u < RS; ++u) {
+        den[u] = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) wv[b][e] = 0;
-      auto step1 = [&](auto pc, int k) __attribute__((always_inline)) {
-        constexpr int P = decltype(pc)::value;
-        const int t = ta + k;
-        const bool vnext = k + 1 < n1;
+        for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) wv[u][b][e] = 0;
+      }
+      constexpr std::integral_constant<int, 0> kEven{};
+      constexpr std::integral_constant<int, 1> kOdd{};
+      for (int t = ta; t < te; ++t) {
         lds_barrier();
-        if (t >= te) {  // uniform: a padding step
-          put_all0(pc);
-          refill0(pc);
-          put_all1(pc, vnext);
-          refill1(pc);
-          return;
-        }
-        u32x4 pb[2];
+        u32x4 pb[RS][2];
         auto weights = [&](auto whole_tag) __attribute__((always_inline)) {
           constexpr bool WHOLE = decltype(whole_tag)::value;
-          scores_of(lds + 2 * P * L::TILEB, [&](auto qc) { put0(pc, qc); }, [&](auto qc, const f32x4& acc)
+          scores_of(lds, [&](auto qc) { put_part(kEven, v_wr, qc); }, [&](auto qc, int u, const f32x4& acc)
                     __attribute__((always_inline)) {
             constexpr int q = decltype(qc)::value, s = q >> 1, h = q & 1;
             float sc[4], w[4];
-            chain_scores(acc, t, q, WHOLE, std::false_type{}, sc);
+            chain_scores(acc, t, u, q, WHOLE, std::false_type{}, sc);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(sc[e] - mrow);
+            for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(sc[e] - mrow[u]);
             if constexpr (FAST) {
 #pragma unroll
               for (int e = 0; e < 4; ++e)  // (the maximum: NaN counts as 0)
-                den = AccT(uint32_t(den) + __float_as_uint(fmaxf(__builtin_fmaf(w[e], a.fxp_scale, kRoundF), kRoundF)));
-              pb[s][2 * h] = p_pack2<DT>(w[0], w[1]);
-              pb[s][2 * h + 1] = p_pack2<DT>(w[2], w[3]);
+                den[u] = AccT(uint32_t(den[u]) + __float_as_uint(fmaxf(__builtin_fmaf(w[e], a.fxp_scale, kRoundF), kRoundF)));
+              pb[u][s][2 * h] = p_pack2<DT>(w[0], w[1]);
+              pb[u][s][2 * h + 1] = p_pack2<DT>(w[2], w[3]);
             } else {
               uint32_t p16[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                den = wadd<BITS>(den, quant<BITS>(__fmul_rn(w[e], a.fxp_scale)));
+                den[u] = wadd<BITS>(den[u], quant<BITS>(__fmul_rn(w[e], a.fxp_scale)));
                 p16[e] = Io<DT>::store(w[e]);
               }
-              pb[s][2 * h] = p16[0] | (p16[1] << 16);
-              pb[s][2 * h + 1] = p16[2] | (p16[3] << 16);
+              pb[u][s][2 * h] = p16[0] | (p16[1] << 16);
+              pb[u][s][2 * h + 1] = p16[2] | (p16[3] << 16);
             }
           });
         };
         if (FAST && tile_whole(t)) weights(std::true_type{});
         else weights(std::false_type{});
-        refill0(pc);
+        refill(st[1]);
 
         // d blocks, the next one's V reads before this one's MFMAs
-        const unsigned char* vt = lds + (2 * P + 1) * L::TILEB;
+        lds_barrier();
+        const unsigned char* vt = lds + RL::TILEB + v_rd;
         u32x2 vr[2][2][2];
         auto issue_v = [&](auto bc) __attribute__((always_inline)) {
           constexpr int b = decltype(bc)::value;
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) vr[b & 1][s][h] = lds_load_tr8(vt + s * 32 * L::ROWB + (vrd[h] ^ (b << 5)));
+            for (int s = 0; s < 2; ++s) vr[b & 1][s][h] = lds_load_tr8(vt + (s * kStepV + h * 4 * RL::PITCH + 32 * b));
         };
-        issue_v(std::integral_constant<int, 0>{});
-        f32x4 accv[FAST ? DBLK : 1];
-        float vmax = 0.0f;
-        static_for<DBLK>([&](auto bc) __attribute__((always_inline)) {
-          constexpr int b = decltype(bc)::value;
-          if constexpr (b + 1 < DBLK) issue_v(std::integral_constant<int, b + 1>{});
-          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        auto blocks = [&](auto&& fn) __attribute__((always_inline)) {
+          issue_v(std::integral_constant<int, 0>{});
+          static_for<DBLK>([&](auto bc) __attribute__((always_inline)) {
+            constexpr int b = decltype(bc)::value;
+            if constexpr (b + 1 < DBLK) issue_v(std::integral_constant<int, b + 1>{});
+            f32x4 acc[RS];
 #pragma unroll
-          for (int s = 0; s < 2; ++s)
-            acc = TR::mma(u32x4{vr[b & 1][s][0][0], vr[b & 1][s][0][1], vr[b & 1][s][1][0], vr[b & 1][s][1][1]}, pb[s], acc);
-          if constexpr (b < 4) put1(pc, bc, vnext);
+            for (int u = 0; u < RS; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int u = 0; u < RS; ++u)
+                acc[u] = TR::mma(u32x4{vr[b & 1][s][0][0], vr[b & 1][s][0][1], vr[b & 1][s][1][0], vr[b & 1][s][1][1]},
+                                 pb[u][s], acc[u]);
+            fn(bc, acc);
+            __builtin_amdgcn_sched_barrier(0);
+          });
+        };
+        auto term = [&](float x) { return __float_as_uint(__builtin_fmaf(x, a.fxp_scale, kRoundF)); };
+        float vmax = 0.0f;
+        f32x4 prev[RS];
+        auto add_terms = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+          for (int u = 0; u < RS; ++u) {
+            vmax = absmax4(vmax, prev[u]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) wv[u][b][e] = AccT(uint32_t(wv[u][b][e]) + term(prev[u][e]));
+          }
+        };
+        blocks([&](auto bc, const f32x4 (&acc)[RS]) __attribute__((always_inline)) {
+          constexpr int b = decltype(bc)::value;
+          if constexpr (b < 4) put_part(kOdd, k_wr, bc);
           if constexpr (FAST) {
             // block b - 1's terms while block b's MFMAs run
-            accv[b] = acc;
-            if constexpr (b > 0) vmax = absmax4(vmax, accv[b - 1]);
+            if constexpr (b > 0) add_terms(b - 1);
+#pragma unroll
+            for (int u = 0; u < RS; ++u) prev[u] = acc[u];
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) wv[b][e] = wadd<BITS>(wv[b][e], quant<BITS>(__fmul_rn(acc[e], a.fxp_scale)));
+            for (int u = 0; u < RS; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) wv[u][b][e] = wadd<BITS>(wv[u][b][e], quant<BITS>(__fmul_rn(acc[u][e], a.fxp_scale)));
           }
-          __builtin_amdgcn_sched_barrier(0);
         });
-        refill1(pc);
+        refill(st[0]);
         if constexpr (FAST) {
-          vmax = absmax4(vmax, accv[DBLK - 1]);
-          auto term = [&](float x) { return __float_as_uint(__builtin_fmaf(x, a.fxp_scale, kRoundF)); };
+          add_terms(DBLK - 1);
+          if (__builtin_amdgcn_ballot_w64(!(vmax < m.vlim)) != 0) {  // uniform: out of the constant's range
+            blocks([&](auto bc, const f32x4 (&acc)[RS]) __attribute__((always_inline)) {
+              constexpr int b = decltype(bc)::value;
+#pragma unroll
+              for (int u = 0; u < RS; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const AccT without = AccT(uint32_t(wv[u][b][e]) - term(acc[u][e]));
+                  wv[u][b][e] = AccT(uint32_t(wadd<BITS>(without, quant<BITS>(__fmul_rn(acc[u][e], a.fxp_scale)))) + kRound);
+                }
+            });
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < RS; ++u) {
+        if constexpr (FAST) {
+          const uint32_t terms = uint32_t(te - ta) * kRound;
+          den[u] = AccT(uint32_t(den[u]) - 16u * terms);
 #pragma unroll
           for (int b = 0; b < DBLK; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) wv[b][e] = AccT(uint32_t(wv[b][e]) + term(accv[b][e]));
-          if (__builtin_amdgcn_ballot_w64(!(vmax < m.vlim)) != 0) {  // uniform: out of the constant's range
+            for (int e = 0; e < 4; ++e) wv[u][b][e] = AccT(uint32_t(wv[u][b][e]) - terms);
+        }
+        den[u] = wadd<BITS>(den[u], __shfl_xor(den[u], 16, 64));
+        den[u] = wadd<BITS>(den[u], __shfl_xor(den[u], 32, 64));
+        if (SPLIT && split > 0) {  // uniform
+          store_record(u, c, mx[u], den[u], wv[u]);
+        } else if (__builtin_amdgcn_ballot_w64(Mr[u] != -__builtin_inff()) == 0) {
+          // nothing folded yet in the wave: the chunk's own sums
+#pragma unroll
+          for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) Wr[u][b][e] = wv[u][b][e];
+          Dr[u] = den[u];
+          Mr[u] = mx[u];
+        } else if (mx[u] != -__builtin_inff()) {
+          float Mn, fa, fb;
+          merge_factors(Mr[u], mx[u], Mn, fa, fb);
+          // fa or fb is 1 (unless both maxima are +inf), and rescale(x, 1) = x for
+          // 16- and 32-bit sums: one side is rescaled
+          const bool one_a = fa == 1.0f;
+          if (BITS != 64 && __builtin_amdgcn_ballot_w64(!(one_a || fb == 1.0f)) == 0) {
+            const float f = one_a ? fb : fa;
+            Dr[u] = wadd<BITS>(rescale<BITS>(one_a ? den[u] : Dr[u], f), one_a ? Dr[u] : den[u]);
 #pragma unroll
             for (int b = 0; b < DBLK; ++b)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const AccT without = AccT(uint32_t(wv[b][e]) - term(accv[b][e]));
-                wv[b][e] = AccT(uint32_t(wadd<BITS>(without, quant<BITS>(__fmul_rn(accv[b][e], a.fxp_scale)))) + kRound);
+                const AccT x = one_a ? wv[u][b][e] : Wr[u][b][e], y = one_a ? Wr[u][b][e] : wv[u][b][e];
+                Wr[u][b][e] = wadd<BITS>(rescale<BITS>(x, f), y);
               }
+          } else {
+            Dr[u] = wadd<BITS>(rescale<BITS>(Dr[u], fa), rescale<BITS>(den[u], fb));
+#pragma unroll
+            for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                Wr[u][b][e] = wadd<BITS>(rescale<BITS>(Wr[u][b][e], fa), rescale<BITS>(wv[u][b][e], fb));
           }
+          Mr[u] = Mn;
         }
-      };
-      for (int k = 0; k < n1; k += 2) {
-        step1(std::integral_constant<int, 0>{}, k);
-        step1(std::integral_constant<int, 1>{}, k + 1);
-      }
-      if constexpr (FAST) {
-        const uint32_t terms = uint32_t(te - ta) * kRound;
-        den = AccT(uint32_t(den) - 16u * terms);
-#pragma unroll
-        for (int b = 0; b < DBLK; ++b)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) wv[b][e] = AccT(uint32_t(wv[b][e]) - terms);
-      }
-      den = wadd<BITS>(den, __shfl_xor(den, 16, 64));
-      den = wadd<BITS>(den, __shfl_xor(den, 32, 64));
-      if (SPLIT && split > 0) {  // uniform
-        store_record(c, mx, den, wv);
-      } else if (__builtin_amdgcn_ballot_w64(Mr != -__builtin_inff()) == 0) {
-        // nothing folded yet in the wave: the chunk's own sums
-#pragma unroll
-        for (int b = 0; b < DBLK; ++b)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) Wr[b][e] = wv[b][e];
-        Dr = den;
-        Mr = mx;
-      } else if (mx != -__builtin_inff()) {
-        float Mn, fa, fb;
-        merge_factors(Mr, mx, Mn, fa, fb);
-        // fa or fb is 1 (unless both maxima are +inf), and rescale(x, 1) = x for
-        // 16- and 32-bit sums: one side is rescaled
-        const bool one_a = fa == 1.0f;
-        if (BITS != 64 && __builtin_amdgcn_ballot_w64(!(one_a || fb == 1.0f)) == 0) {
-          const float f = one_a ? fb : fa;
-          Dr = wadd<BITS>(rescale<BITS>(one_a ? den : Dr, f), one_a ? Dr : den);
-#pragma unroll
-          for (int b = 0; b < DBLK; ++b)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const AccT x = one_a ? wv[b][e] : Wr[b][e], y = one_a ? Wr[b][e] : wv[b][e];
-              Wr[b][e] = wadd<BITS>(rescale<BITS>(x, f), y);
-            }
-        } else {
-          Dr = wadd<BITS>(rescale<BITS>(Dr, fa), rescale<BITS>(den, fb));
-#pragma unroll
-          for (int b = 0; b < DBLK; ++b)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) Wr[b][e] = wadd<BITS>(rescale<BITS>(Wr[b][e], fa), rescale<BITS>(wv[b][e], fb));
-        }
-        Mr = Mn;
       }
     }
   }
-
-  if constexpr (SPLIT) {
-    if (split == 0) {
-      if (c_lo < c_hi) store_record(c_hi - 1, Mr, Dr, Wr);
-      if (me.valid && kg == 0) {
-        int* cr = a.crange + 2 * (me.token * a.num_heads + me.head);
-        cr[0] = c_lo < c_hi ? c_hi - 1 : c_first;
-        cr[1] = c_end;
+#pragma unroll
+  for (int u = 0; u < RS; ++u) {
+    const RowInfo me = row_of(u);
+    if constexpr (SPLIT) {
+      if (split == 0) {
+        if (c_lo < c_hi) store_record(u, c_hi - 1, Mr[u], Dr[u], Wr[u]);
+        if (me.valid && kg == 0) {
+          int* cr = a.crange + 2 * (me.token * a.num_heads + me.head);
+          cr[0] = c_lo < c_hi ? c_hi - 1 : c_first;
+          cr[1] = c_end;
+        }
       }
+    } else if (me.valid) {
+      // the row's quotients over one denominator by its rounded reciprocal: the
+      // bits of div_rn
+      const float den_f = fmaxf(acc_f32<BITS>(Dr[u], a.fxp_inv), 1.0e-6f);
+      const float rcp = div_rn(1.0f, den_f);
+      T* orow = static_cast<T*>(a.o) + me.token * a.so_t + int64_t(me.head) * a.so_h;
+#pragma unroll
+      for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float num = acc_f32<BITS>(Wr[u][b][e], a.fxp_inv);
+          orow[b * 16 + 4 * kg + e] = Io<DT>::store(BITS == 64 ? div_rn(num, den_f) : div_rn_by_recip(num, den_f, rcp));
+        }
     }
-  } else if (me.valid) {
-    // the row's quotients over one denominator by its rounded reciprocal: the
-    // bits of div_rn
-    const float den_f = fmaxf(acc_f32<BITS>(Dr, a.fxp_inv), 1.0e-6f);
-    const float rcp = div_rn(1.0f, den_f);
-    T* orow = static_cast<T*>(a.o) + me.token * a.so_t + int64_t(me.head) * a.so_h;
-#pragma unroll
-    for (int b = 0; b < DBLK; ++b)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float num = acc_f32<BITS>(Wr[b][e], a.fxp_inv);
-        orow[b * 16 + 4 * kg + e] = Io<DT>::store(BITS == 64 ? div_rn(num, den_f) : div_rn_by_recip(num, den_f, rcp));
-      }
   }
 }
 
@@ -1378,9 +1415,9 @@ template <int BITS> bool fast_of(const AttnArgs& a) {
 }
 
 template <int DT, int BITS, int D, bool SPLIT, bool FAST, bool CAP>
-int launch_rows64(const Mx4Args& m, dim3 grid, hipStream_t st) {
-  auto kern = attn_mx4_rows64_kernel<DT, BITS, D, SPLIT, FAST, CAP>;
-  constexpr int lds = 4 * Lds<D>::TILEB;
+int launch_prompt(const Mx4Args& m, dim3 grid, hipStream_t st) {
+  auto kern = attn_mx4_prompt_kernel<DT, BITS, D, SPLIT, FAST, CAP, row_sets(BITS, D)>;
+  constexpr int lds = 2 * PromptLds<D>::TILEB;
   static bool attr_done = false;  // benign race: the attribute is idempotent
   if (!attr_done) {
     const hipError_t e =
@@ -1392,13 +1429,13 @@ int launch_rows64(const Mx4Args& m, dim3 grid, hipStream_t st) {
   return 0;
 }
 
-template <int DT, int BITS, int D, bool SPLIT> int launch_rows64(const Mx4Args& m, dim3 grid, hipStream_t st) {
+template <int DT, int BITS, int D, bool SPLIT> int launch_prompt(const Mx4Args& m, dim3 grid, hipStream_t st) {
   if constexpr (BITS != 64) {
     if (fast_of<BITS>(m.a))
-      return m.a.softcap_log2 > 0.0f ? launch_rows64<DT, BITS, D, SPLIT, true, true>(m, grid, st)
-                                     : launch_rows64<DT, BITS, D, SPLIT, true, false>(m, grid, st);
+      return m.a.softcap_log2 > 0.0f ? launch_prompt<DT, BITS, D, SPLIT, true, true>(m, grid, st)
+                                     : launch_prompt<DT, BITS, D, SPLIT, true, false>(m, grid, st);
   }
-  return launch_rows64<DT, BITS, D, SPLIT, false, false>(m, grid, st);
+  return launch_prompt<DT, BITS, D, SPLIT, false, false>(m, grid, st);
 }
 
 template <int DT, int BITS, int D, bool SPLIT, int MAXE> void launch_rows16(const Mx4Args& m, dim3 grid, hipStream_t st) {
@@ -1425,25 +1462,26 @@ int launch_mx4(Mx4Args m, const Mx4Plan& p, int num_requests, int max_query_len,
   const int64_t max_rows = int64_t(max_query_len > 1 ? max_query_len : 1) * a.group;
   const bool split = p.splits > 1 || p.pq_splits > 1;
   int64_t qtiles = cdiv(max_rows, QROWS);
-  if (p.rows64) {
+  if (p.prompt) {
     a.pq_rows = kPrefillRows;
     qtiles = std::min<int64_t>(qtiles, kShortTiles);
-    const int64_t ptiles = cdiv(max_rows, PQROWS);
+    constexpr int kRows = row_sets(BITS, D) * PQROWS;
+    const int64_t ptiles = cdiv(max_rows, kRows);
     // a flat grid over the tokens where requests x the longest one's tiles
     // would be mostly empty
-    const int64_t flat = num_tokens * a.group / PQROWS + num_requests;
+    const int64_t flat = num_tokens * a.group / kRows + num_requests;
     dim3 grid(unsigned(num_requests * a.num_kv_heads), unsigned(ptiles), unsigned(p.pq_splits));
     if (ptiles > 65535 || (num_requests * ptiles - flat) * a.num_kv_heads * p.pq_splits > kFlatEmpty) {
       a.pq_blocks = int(flat);
       grid = dim3(unsigned(flat * a.num_kv_heads), 1, unsigned(p.pq_splits));
     }
-    const int e = p.pq_splits > 1 ? launch_rows64<DT, BITS, D, true>(m, grid, st)
-                                  : launch_rows64<DT, BITS, D, false>(m, grid, st);
+    const int e = p.pq_splits > 1 ? launch_prompt<DT, BITS, D, true>(m, grid, st)
+                                  : launch_prompt<DT, BITS, D, false>(m, grid, st);
     if (e) return e;
   }
   const dim3 grid(unsigned(num_requests * a.num_kv_heads), unsigned(qtiles), unsigned(p.splits));
   // (rows of the longest request that these workgroups can get)
-  const int64_t short_rows = p.rows64 ? kPrefillRows - 1 : max_rows;
+  const int64_t short_rows = p.prompt ? kPrefillRows - 1 : max_rows;
   launch_rows16<DT, BITS, D>(m, grid, split, short_rows <= 4 ? 1 : short_rows <= 8 ? 2 : 4, st);
   if (!split) return launch_status();
   const int64_t ws_rows = a.tok_cap > 0 ? int64_t(num_requests) * a.tok_cap : num_tokens;
