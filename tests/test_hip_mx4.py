@@ -328,6 +328,26 @@ def test_attention_formula_and_float_cache_bits(shape):
         assert torch.equal(b.run(splits), want), splits
 
 
+@pytest.mark.parametrize("m,ctx,window", [(12, 513, 0), (33, 1537, 0), (48, 577, 70), (129, 1100, 600), (32, 1024, 481),
+                                          (70, 1664, 513), (31, 62, 3), (200, 2111, 1024), (64, 640, 65)])
+def test_prompts_whose_first_and_last_chunks_are_partly_live(m, ctx, window):
+    # one to eight live tiles at either end of a row tile's keys, even and odd, over one to five chunks
+    b = Batch([(m, ctx), (1, 40), (m + 5, ctx + 64)], 8, 2, 128, 16, BF, seed=ctx)
+    for kw in (dict(window=window), dict(window=window, causal=False), dict(window=window, softcap=5.0)):
+        want = b.over_floats(**kw)
+        for splits in (0, 1, 2, 3):
+            assert torch.equal(b.run(splits, **kw), want), (kw, splits)
+
+
+@pytest.mark.parametrize("d,dtype", [(128, HF), (256, BF)])
+def test_one_prompt_beside_many_decode_steps(d, dtype):
+    # requests x the longest one's row tiles are mostly empty: the grid follows the tokens instead
+    b = Batch([(1, 3 + 7 * i) for i in range(90)] + [(900, 1000)] + [(1, 33), (0, 5), (40, 50)], 8, 2, d, 16, dtype, seed=8)
+    want = b.over_floats()
+    for splits in (0, 1, 2):
+        assert torch.equal(b.run(splits), want), splits
+
+
 OPTIONS = [dict(softcap=3.0), dict(window=1), dict(window=100), dict(window=700), dict(causal=False), dict(scale=0.3),
            dict(alibi=True), dict(alibi=True, softcap=20.0, window=600), dict(causal=False, window=50)]
 
