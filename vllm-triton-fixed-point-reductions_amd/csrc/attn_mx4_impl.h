@@ -1247,18 +1247,19 @@ __global__ __launch_bounds__(kPThreads, D == 256 ? 1 : 2) void attn_mx4_prompt_k
 // order. A row's records are loaded a batch ahead of their use.
 //
 // A wave takes a row, D / 64 elements a lane, or (WIDE, for launches of few rows
-// of many chunks) the four waves of a workgroup take 64 elements of a row: wave 0
-// the chunks of a block of 64 up to the last one that raises the maximum, then
-// each a quarter of the rest. One request over 131072 keys, 32 rows of 256
-// records: 43 us with a thread folding step by step, 21.6 with a wave a row, 9
-// with four (WIDE).
+// of many chunks) the four waves of a workgroup take 64 elements of a row, each a
+// quarter of every block of 64 chunks: a wave leaves its sums up to each chunk
+// that raises the maximum, and wave 0 rescales and adds those in order. One
+// request over 131072 keys, 32 rows of 256 records: 43 us with a thread folding
+// step by step, 21.6 with a wave a row, 19.3 with four of which wave 0 folds up to
+// the last raise alone, 10.8 so.
 template <int DT, int BITS, int D, bool WIDE>
 __global__ __launch_bounds__(256) void attn_mx4_combine_kernel(AttnArgs a) {
   using T = typename Traits<DT>::T;
   using AccT = typename AccOf<BITS>::T;
   constexpr int V = WIDE ? 1 : D / 64, PARTS = WIDE ? D / 64 : 1;
   typedef AccT accv __attribute__((ext_vector_type(V)));
-  __shared__ AccT part_w[WIDE ? 4 : 1][64];
+  __shared__ AccT part_w[WIDE ? 68 : 1][64];  // up to chunk l of the block; the waves' last sums
   const int lane = threadIdx.x & 63;
   const int wave = WIDE ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const uint32_t unit =
@@ -1296,26 +1297,22 @@ __global__ __launch_bounds__(256) void attn_mx4_combine_kernel(AttnArgs a) {
 #pragma unroll
     for (int k = 0; k < NB; ++k) w[k] = *reinterpret_cast<const accv*>(wv_p + int64_t(min(cb + k, c1 - 1)) * D);
   };
-  // the waves' sums of added terms into wave 0's
-  auto gather = [&]() __attribute__((always_inline)) {
-    if constexpr (WIDE) {
-      part_w[wave][lane] = W[0];
-      __syncthreads();
-      if (wave == 0) {
-        W[0] = wadd<BITS>(wadd<BITS>(part_w[0][lane], part_w[1][lane]), wadd<BITS>(part_w[2][lane], part_w[3][lane]));
-      } else {
-        W[0] = 0;
-      }
-      __syncthreads();
-    }
+  float mn = -__builtin_inff();  // the lane's record of the next block
+  AccT dn = 0;
+  auto load_lane = [&](int cb) __attribute__((always_inline)) {
+    const int cl = min(cb + lane, c1 - 1);
+    mn = pm_p[cl];
+    dn = den_p[cl];
   };
+  if (c0 < c1) {
+    load(c0 + wave * (WIDE ? NB : 0), wc[0]);
+    load_lane(c0);
+  }
   for (int cs = c0; cs < c1; cs += 64) {
-    if constexpr (WIDE) load(cs + wave * NB, wc[0]);
-    else load(cs, wc[0]);
     // this lane's chunk: its maximum, and the factors of its fold
-    const int cl = min(cs + lane, c1 - 1);
-    const float mc = cs + lane < c1 ? pm_p[cl] : -__builtin_inff();
-    const AccT dc = den_p[cl];
+    const float mc = cs + lane < c1 ? mn : -__builtin_inff();
+    const AccT dc = dn;
+    if (cs + 64 < c1) load_lane(cs + 64);
     float incl = mc;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -1345,12 +1342,12 @@ __global__ __launch_bounds__(256) void attn_mx4_combine_kernel(AttnArgs a) {
         return AccT(__builtin_amdgcn_readlane(int(dr), l));
       }
     };
-    // chunks k0 .. of the block in order, up to chunk `last`
-    auto fold = [&](int k0, int last, const accv (&w)[NB]) __attribute__((always_inline)) {
+    // chunks k0 .. of the block in order
+    auto fold = [&](int k0, const accv (&w)[NB]) __attribute__((always_inline)) {
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
         const int l = k0 + k;  // uniform
-        if (l > last || !((seen >> l) & 1)) continue;
+        if (!((seen >> l) & 1)) continue;
         if ((moves >> l) & 1) {
           const float g = __uint_as_float(uint32_t(__builtin_amdgcn_readlane(int(__float_as_uint(fa)), l)));
 #pragma unroll
@@ -1362,38 +1359,62 @@ __global__ __launch_bounds__(256) void attn_mx4_combine_kernel(AttnArgs a) {
       }
     };
     if constexpr (WIDE) {
-      const int last = moves ? 63 - __builtin_clzll(moves) : -1;  // uniform, and the same in every wave
-      if (last >= 0) {
-        gather();
-        if (wave == 0) {
-          for (int h = 0; h * NB <= last; ++h) {
-            load(cs + h * NB, wc[1]);
-            fold(h * NB, last, wc[1]);
+      // the wave's quarter: a sum per run of chunks between those that move
+      auto quarter = [&](const accv (&w)[NB]) __attribute__((always_inline)) {
+        AccT sum = 0;
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+          const int l = wave * NB + k;  // uniform
+          if ((moves >> l) & 1) {
+            part_w[l][lane] = sum;
+            sum = 0;
           }
+          const float f = __uint_as_float(uint32_t(__builtin_amdgcn_readlane(int(__float_as_uint(fb)), l)));
+          if ((seen >> l) & 1) sum = wadd<BITS>(sum, rescale<BITS>(w[k][0], f));
         }
+        part_w[64 + wave][lane] = sum;
+      };
+      if ((cs - c0) & 64) {
+        if (cs + 64 < c1) load(cs + 64 + wave * NB, wc[0]);
+        quarter(wc[1]);
+      } else {
+        if (cs + 64 < c1) load(cs + 64 + wave * NB, wc[1]);
+        quarter(wc[0]);
       }
-      // the rest of the block: a quarter each
-#pragma unroll
-      for (int k = 0; k < NB; ++k) {
-        const int l = wave * NB + k;
-        if (l > last && ((seen >> l) & 1)) term(l, wc[0][k]);
-      }
+      __syncthreads();
       if (wave == 0) {
-        AccT t = lane > last && ((seen >> lane) & 1) ? dr : AccT(0);
+        // the denominators' sums up to the lane's chunk, its own included
+        AccT sum = (seen >> lane) & 1 ? dr : AccT(0);
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) t = wadd<BITS>(t, __shfl_xor(t, o, 64));
-        Dn = wadd<BITS>(Dn, t);
+        for (int o = 1; o < 64; o <<= 1) {
+          const AccT x = __shfl_up(sum, o, 64);
+          if (lane >= o) sum = wadd<BITS>(sum, x);
+        }
+        auto minus = [](AccT x, AccT y) { return AccT(uint64_t(x) - uint64_t(y)); };
+        AccT done = 0;
+        int q = 0;  // the quarter whose sums are being added
+        for (uint64_t todo = moves; todo; todo &= todo - 1) {
+          const int l = __builtin_ctzll(todo);
+          for (; q < l / NB; ++q) W[0] = wadd<BITS>(W[0], part_w[64 + q][lane]);
+          const float g = __shfl(fa, l, 64);
+          W[0] = rescale<BITS>(wadd<BITS>(W[0], part_w[l][lane]), g);
+          const AccT upto = l > 0 ? __shfl(sum, l - 1, 64) : AccT(0);
+          Dn = rescale<BITS>(wadd<BITS>(Dn, minus(upto, done)), g);
+          done = upto;
+        }
+        for (; q < 4; ++q) W[0] = wadd<BITS>(W[0], part_w[64 + q][lane]);
+        Dn = wadd<BITS>(Dn, minus(__shfl(sum, 63, 64), done));
       }
+      __syncthreads();
     } else {
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
         if (cs + h * NB >= c1) break;  // uniform
-        if (h + 1 < NH && cs + (h + 1) * NB < c1) load(cs + (h + 1) * NB, wc[(h + 1) & 1]);
-        fold(h * NB, 63, wc[h & 1]);
+        if (cs + (h + 1) * NB < c1) load(cs + (h + 1) * NB, wc[(h + 1) & 1]);
+        fold(h * NB, wc[h & 1]);
       }
     }
   }
-  gather();
   if (wave != 0) return;
   const float den_f = fmaxf(acc_f32<BITS>(Dn, a.fxp_inv), 1.0e-6f);
   T* o = static_cast<T*>(a.o) + token * a.so_t + int64_t(head) * a.so_h + d;
