@@ -20,18 +20,20 @@ struct Planned {
   WsLayout ws;
 };
 
-// Split policy (bf16, 32 query heads over 8 kv heads of size 128; a chunk is
-// 512 keys).
+// Split policy (bf16, 32 query heads over 8 kv heads of size 128, the cache as
+// empty_cache lays it out; a chunk is 512 keys).
 // 16-row workgroups split when there are chunks to hand out and the launch is
-// small or its lengths may differ: up to 256 workgroups from two chunks on
-// (16 requests of 2000 keys 20 us, unsplit 25; 4 of 1000 11.8 against 13.6),
-// up to 1024 from four (64 requests of 250 .. 2000 keys 37 us, unsplit 43; all
-// of 2000 56 against 53.5), up to 2048 beyond four (256 requests of
-// 1000 .. 8000 keys 427 us, unsplit 452; all of 8000 758 against 741).  About
-// 6144 workgroups, eight rounds of the card, even the lengths out (64 requests
-// of 16000 keys: 12 splits 381 us, 8 400, 32 388); a request alone has its
-// records read by one workgroup per row, which ends the gain at 128 (64000
-// keys 40.9 us, 64 splits 42.3; over one kv head 18.0 against 22.5).
+// small, or its lengths may differ and it is not large (a split leaves a record
+// per chunk): up to 128 workgroups from two chunks on (16 requests of 1000 keys
+// 11.7 us, unsplit 12.4; 24 of them 14.1 against 12.7), up to 1024 from four (64
+// requests of 1000 .. 8000 keys 70 us, unsplit 104; all of 8000 121 against 114;
+// 128 of 500 .. 4000 76 against 84, all of 4000 125 against 113), none beyond
+// (256 requests of 1000 .. 8000 keys 278 us, unsplit 261; all of 8000 493 against
+// 398). About 6144 workgroups, eight rounds of the card, even the lengths out,
+// and 12 splits where that is fewer (64 requests of 2000 .. 16000 keys: 12 splits
+// 145 us, 4 160, 32 145; 128 of 1000 .. 8000 12 splits 138, 8 144); beyond 128 a
+// request alone gains nothing (64000 keys 24.3 us, 64 splits 24.9; over one kv
+// head 13.7 against 18.1).
 // The prompts' workgroups (128 rows) split while fewer than two fall to a CU,
 // and up to that: 512 new tokens over 4096 keys 94 us with 4 splits, 205 unsplit,
 // 97 with 8; 128 over 16000 97 us with 16, 788 unsplit; 4 x 256 over 4096 180 us
@@ -54,8 +56,8 @@ Planned plan_mx4(int num_requests, int64_t num_tokens, int num_heads, int num_kv
     s16 = sp = std::min<int64_t>({int64_t(requested), slots, kMaxGridZ});
   } else {
     const bool only_long = r.p.prompt && num_tokens == int64_t(num_requests) * max_query_len;
-    const int64_t most = chunks < 4 ? 256 : chunks == 4 ? 1024 : 2048;
-    if (wgs16 <= most && !only_long) s16 = std::min(chunks, std::clamp<int64_t>(6144 / wgs16, 8, 128));
+    if (wgs16 <= (chunks < 4 ? 128 : 1024) && !only_long)
+      s16 = std::min(chunks, std::clamp<int64_t>(6144 / wgs16, 12, 128));
     if (r.p.prompt && wgsp < 512) sp = std::min(cdiv(512, wgsp), chunks);
   }
   auto layout = [&](int64_t rows) { return ws_layout(rows, num_heads, head_dim, int_bits, true, slots); };
