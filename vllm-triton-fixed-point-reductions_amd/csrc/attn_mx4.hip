@@ -33,7 +33,10 @@ struct Planned {
 // and 12 splits where that is fewer (64 requests of 2000 .. 16000 keys: 12 splits
 // 145 us, 4 160, 32 145; 128 of 1000 .. 8000 12 splits 138, 8 144); beyond 128 a
 // request alone gains nothing (64000 keys 24.3 us, 64 splits 24.9; over one kv
-// head 13.7 against 18.1).
+// head 13.7 against 18.1). A window evens the lengths by itself: up to 384
+// workgroups (the last where equal lengths gain: 48 requests of 4000 keys 51 us,
+// unsplit 58; 83 requests under a window of 1024, f16, head size 64: 26.2 us,
+// unsplit 24.0).
 // The prompts' workgroups (128 rows) split while fewer than two fall to a CU,
 // and up to that: 512 new tokens over 4096 keys 94 us with 4 splits, 205 unsplit,
 // 97 with 8; 128 over 16000 97 us with 16, 788 unsplit; 4 x 256 over 4096 180 us
@@ -56,7 +59,7 @@ Planned plan_mx4(int num_requests, int64_t num_tokens, int num_heads, int num_kv
     s16 = sp = std::min<int64_t>({int64_t(requested), slots, kMaxGridZ});
   } else {
     const bool only_long = r.p.prompt && num_tokens == int64_t(num_requests) * max_query_len;
-    if (wgs16 <= (chunks < 4 ? 128 : 1024) && !only_long)
+    if (wgs16 <= (chunks < 4 ? 128 : window > 0 ? 384 : 1024) && !only_long)
       s16 = std::min(chunks, std::clamp<int64_t>(6144 / wgs16, 12, 128));
     if (r.p.prompt && wgsp < 512) sp = std::min(cdiv(512, wgsp), chunks);
   }
