@@ -451,9 +451,10 @@ int fxpr_gather_cache_mx4(
  * bits as over a cache of io_dtype (f16 / bf16) that holds the values the codes
  * stand for, so outputs are bitwise independent of the split count, of the
  * batch and of max_query_len. page_size: a power of two, 16 or more. q rows
- * 16-byte aligned. The launch needs a workspace of fxpr_attention_mx4_plan()
- * bytes when that is non-zero (no zeroing). num_kv_splits: 0 = automatic. No
- * counterpart in the reference.
+ * 16-byte aligned. Keys past the max_blocks_per_seq * page_size of a table row
+ * are not there. The launch needs a workspace of fxpr_attention_mx4_plan() bytes,
+ * 16-byte aligned, when that is non-zero (no zeroing). num_kv_splits: 0 =
+ * automatic. No counterpart in the reference.
  */
 int fxpr_unified_attention_mx4(
     const void* q, const void* codes, const void* scales, void* o, int io_dtype,

@@ -445,6 +445,58 @@ def test_bad_tables_stay_inside_the_cache():
     assert bool(torch.isfinite(b.run().float()).all())
 
 
+def test_a_table_shorter_than_the_sequences():
+    # keys past the table's are not there, however the keys are split; lengths and starts of any value stay inside
+    b = Batch([(1, 1700), (60, 900), (2, 1200)], 8, 2, 128, 16, BF, seed=13)
+    b.table = b.table[:, :40].contiguous()
+    want = b.run(1)
+    for splits in (0, 2, 5):
+        assert torch.equal(b.run(splits), want), splits
+    b.lens = torch.tensor([700, 900, 700], dtype=torch.int32)  # request 2's new tokens lie past the table: 640 keys
+    b.lens[2] = 640 + 2
+    o = b.run(1)
+    b.lens = torch.tensor([(1 << 31) - 1, 900, (1 << 31) - 1], dtype=torch.int32)
+    for splits in (0, 1, 2):
+        for window in (0, 100):
+            assert bool(torch.isfinite(b.run(splits, window=window).float()).all())
+        far = b.run(splits)
+        assert torch.equal(far[1:61], o[1:61]) and torch.equal(far[61:], o[61:])  # every key of the table is seen
+    b.lens = torch.tensor([-5, 900, -1000], dtype=torch.int32)
+    for splits in (0, 1, 2):
+        far = b.run(splits)
+        assert not far[0].any() and not far[61:].any() and torch.equal(far[1:61], o[1:61])
+
+
+def test_rows_of_infinities_and_nan():
+    # such rows are the float cache's, and the others do not change
+    b = Batch([(1, 700), (40, 600), (3, 90)], 8, 2, 128, 16, BF, seed=12)
+    base = b.run()
+    bad = {0: (2, math.inf), 5: (0, math.nan), 10: (7, -math.inf), 20: (3, torch.finfo(BF).max), 42: (1, math.nan)}
+    for row, (head, v) in bad.items():
+        b.q[row, head, :: 2 if math.isinf(v) else 1] = v
+    want = b.over_floats().view(torch.int16)
+    for splits in (0, 1, 2):
+        o = b.run(splits)
+        assert torch.equal(o.view(torch.int16), want), splits
+        for row, (head, _) in bad.items():
+            o[row, head] = base[row, head]
+        assert torch.equal(o, base)
+
+
+def test_a_strided_output_keeps_the_rows_of_no_request():
+    b = Batch([(1, 20), (2, 30)], 4, 2, 64, 16, HF, seed=9)
+    want = b.run()
+    n = b.q.shape[0]
+    b.q = torch.cat([b.q, randn(5, 4, 64, dtype=HF)])
+    wide = torch.full((n + 5, 4, 128), 7.0, dtype=HF, device="cuda")
+    b.run(o=wide[:, :, ::2])
+    assert torch.equal(wide[:n, :, ::2], want) and bool((wide[n:] == 7).all()) and bool((wide[:, :, 1::2] == 7).all())
+    wide.fill_(7.0)
+    mx4.unified_attention_run(b.q.cuda(), b.codes, b.scales, wide[:, :, ::2], b.qsl.cuda(), b.lens.cuda(), b.table.cuda(),
+                              b.max_q, None, True, None, 32, 16, 0.0, 0, 0)
+    assert torch.equal(wide[:n, :, ::2], want) and bool((wide[n:] == 7).all())
+
+
 @pytest.mark.parametrize("order", ["heads", "slots"])
 def test_strides(order):
     # q, o and the table as views; the cache in another order, one layer of a stack of caches

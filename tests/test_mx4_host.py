@@ -172,6 +172,16 @@ def test_c_abi_refusals_cache():
     assert write(nb=0) == 0  # no slot exists: every one is padding
 
 
+def test_c_abi_refuses_what_its_indices_do_not_hold():
+    lib = _hip.load()
+    for t, h in (((1 << 30) + 1, 1), ((1 << 29) + 1, 2), ((1 << 26) + 1, 16)):
+        assert lib.fxpr_gather_cache_mx4(P, P, P, P, 1, P, t, h, 128, 16, 8, 4096, 2048, 128, 64, 256, 128, 8, 4, None) == -3
+        assert lib.fxpr_reshape_and_cache_mx4(P, P, P, P, 1, P, t, h, 128, 16, 8, 0, 0, 0, 0, 4096, 2048, 128, 64, 256, 128,
+                                              8, 4, None) == -3
+    need = lib.fxpr_attention_mx4_plan(1, 1, 8, 2, 128, 16, 1, 4096, 0, 32, 4, None)
+    assert _attn(mb=4096, splits=4, ws=ctypes.c_void_p(264), wsb=need) == -4  # not 16-byte aligned
+
+
 def plan(reqs, tokens, hq, hk, d, page, mq, mb, window=0, bits=32, splits=0):
     out = (ctypes.c_int32 * 4)()
     n = _hip.load().fxpr_attention_mx4_plan(reqs, tokens, hq, hk, d, page, mq, mb, window, bits, splits, out)

@@ -151,13 +151,14 @@ extern "C" int fxpr_unified_attention_mx4(
   // (quotient()'s ranges: rows of a request by the group, request x kv head by
   // the kv heads)
   const int64_t group = num_heads / num_kv_heads;
-  if ((std::max(max_rows, num_tokens * group) + 64 * (int64_t(num_requests) + 1)) * group > int64_t(0xffffffff) ||
+  if ((std::max(max_rows, num_tokens * group) + 2 * PQROWS * (int64_t(num_requests) + 1)) * group > int64_t(0xffffffff) ||
       int64_t(num_requests) * num_kv_heads * num_kv_heads > int64_t(0xffffffff))
     return FXPR_E_SHAPE;
   if (max_rows > int64_t(0x7fffffff) ||
       (num_tokens * group / PQROWS + num_requests) * num_kv_heads > int64_t(0x7fffffff))
     return FXPR_E_SHAPE;
-  if (plan.ws.total > 0 && (!workspace || workspace_bytes < plan.ws.total)) return FXPR_E_WORKSPACE;
+  if (plan.ws.total > 0 && (!workspace || workspace_bytes < plan.ws.total || !aligned(workspace, 16)))
+    return FXPR_E_WORKSPACE;
 
   Mx4Args m{};
   AttnArgs& a = m.a;

@@ -211,12 +211,12 @@ struct Pager {
   __device__ __forceinline__ int granule(int g) const { return min(g, last_key >> 4); }
   // the table entry of (clamped) granule g
   __device__ __forceinline__ int entry(int g) const {
-    return row[uint32_t(min((16 * g) >> ps_shift, max_blocks - 1))];
+    return row[min((16u * uint32_t(g)) >> ps_shift, uint32_t(max_blocks - 1))];
   }
   // the same per lane (a vector load), granules of a chunk: any beyond the
   // sequence too (a clamped entry of the table row, never used)
   __device__ __forceinline__ int entry_at(int g) const {
-    return reinterpret_cast<const int32_t*>((uint64_t)row)[uint32_t(min((16 * g) >> ps_shift, max_blocks - 1))];
+    return reinterpret_cast<const int32_t*>((uint64_t)row)[min((16u * uint32_t(g)) >> ps_shift, uint32_t(max_blocks - 1))];
   }
   __device__ __forceinline__ uint32_t block(int e) const { return uint32_t(e < 0 ? 0 : min(e, last_block)); }
   // byte offset of granule g's first row
@@ -234,7 +234,7 @@ struct Pager {
 template <class A> __device__ __forceinline__ Pager make_pager(const A& a, int r, int seq_len) {
   Pager p;
   p.row = (ConstI32)(a.bt + int64_t(r) * a.sbt);
-  p.last_key = max(seq_len - 1, 0);
+  p.last_key = max(seq_len, 1) - 1;
   p.last_block = int(a.num_blocks - 1 < 0x7fffffff ? a.num_blocks - 1 : 0x7fffffff);
   p.max_blocks = a.max_blocks;
   p.ps_shift = a.ps_shift;
@@ -679,6 +679,7 @@ __global__ __launch_bounds__(kThreads, (rows16_wgs<BITS, D, MAXE>())) void attn_
   w.q_len = ((ConstI32)a.qsl)[w.r + 1] - w.q_start;
   w.seq_len = ((ConstI32)a.seq_lens)[w.r];
   w.ctx = w.seq_len - w.q_len;
+  w.seq_len = min(w.seq_len, int(a.lmax));  // keys past the table's are not there
   const int rows_total = w.q_len * a.group;
   w.row0 = blockIdx.y * (MAXE == 4 ? QROWS : 4 * MAXE);
   if (w.row0 >= rows_total) return;                        // uniform
@@ -756,8 +757,8 @@ __global__ __launch_bounds__(kPThreads, D == 256 ? 1 : 2) void attn_mx4_prompt_k
   }
   const int q_start = ((ConstI32)a.qsl)[r];
   const int q_len = ((ConstI32)a.qsl)[r + 1] - q_start;
-  const int seq_len = ((ConstI32)a.seq_lens)[r];
-  const int ctx = seq_len - q_len;
+  const int ctx = ((ConstI32)a.seq_lens)[r] - q_len;
+  const int seq_len = min(((ConstI32)a.seq_lens)[r], int(a.lmax));  // keys past the table's are not there
   const int rows_total = q_len * a.group;
   const int row0 = rtile * ROWS;
   if (row0 >= rows_total || rows_total < a.pq_rows) return;  // uniform
@@ -1439,12 +1440,16 @@ template <int DT, int BITS, int D, bool SPLIT, bool FAST, bool CAP>
 int launch_prompt(const Mx4Args& m, dim3 grid, hipStream_t st) {
   auto kern = attn_mx4_prompt_kernel<DT, BITS, D, SPLIT, FAST, CAP, row_sets(BITS, D)>;
   constexpr int lds = 2 * PromptLds<D>::TILEB;
-  static bool attr_done = false;  // benign race: the attribute is idempotent
-  if (!attr_done) {
-    const hipError_t e =
-        hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if constexpr (lds > 64 * 1024) {
+    static bool done[64] = {};  // by device (benign race: the attribute is idempotent)
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return int(e);
-    attr_done = true;
+    if (dev >= 64 || !done[dev]) {
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      if (e != hipSuccess) return int(e);
+      if (dev < 64) done[dev] = true;
+    }
   }
   kern<<<grid, kPThreads, lds, st>>>(m);
   return 0;

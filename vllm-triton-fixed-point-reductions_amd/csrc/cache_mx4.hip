@@ -198,7 +198,7 @@ int run(bool write, Mx4CacheArgs& a, int dtype, int64_t num_tokens, int num_kv_h
   if (head_size != 64 && head_size != 128 && head_size != 256) return FXPR_E_SHAPE;
   if (num_tokens == 0 || (write && num_blocks == 0)) return FXPR_OK;
   if (!a.key || !a.value || !a.slots || (num_blocks > 0 && (!a.codes || !a.scales))) return FXPR_E_ARG;
-  if (num_tokens > int64_t(0x7fffffff) / num_kv_heads) return FXPR_E_SHAPE;
+  if (num_tokens > (int64_t(1) << 30) / num_kv_heads) return FXPR_E_SHAPE;  // (four 32-bit thread indices a row)
   // 16-byte loads of the codes (a row's D / 2 bytes are whole ones) and of the
   // float rows, D / 32 bytes of scales at once
   const int sb = head_size / 32;

@@ -354,6 +354,8 @@ void check_mx4_cache(const char* what, const Tensor& codes, const Tensor& scales
                     what, ": kv_scales must be (num_blocks, 2, block_size, num_kv_heads, head_size / 32)");
   TORCH_CHECK_VALUE(codes.stride(4) == 1 && scales.stride(4) == 1, what,
                     ": kv_codes and kv_scales must be contiguous along a row");
+  TORCH_CHECK_VALUE(codes.size(2) <= (1 << 30) && codes.size(3) <= (1 << 30), what,
+                    ": block_size and num_kv_heads must be at most 2^30");
 }
 
 template <class... Ts> void check_same_device(const char* what, const Tensor& first, const Ts&... others) {
@@ -470,7 +472,7 @@ void unified_attention_mx4(const Tensor& q_in, const Tensor& codes, const Tensor
                         !(block_table.dim() == 2 && block_table.size(0) < num_requests),
                     "block_table must have a row per request");
   const Tensor q = aligned_rows(q_in);
-  Tensor out = o.stride(2) == 1 ? o : at::empty(o.sizes(), o.options());
+  Tensor out = o.stride(2) == 1 ? o : o.clone(at::MemoryFormat::Contiguous);  // (rows of no request stay as they are)
   Tensor bt = block_table.dim() == 2 ? block_table : block_table.reshape({num_requests, -1});
   if (bt.stride(1) != 1) bt = bt.contiguous();
   const Tensor qsl = query_start_loc.contiguous(), sl = seq_lens.contiguous();
@@ -480,19 +482,21 @@ void unified_attention_mx4(const Tensor& q_in, const Tensor& codes, const Tensor
   const double scale = softmax_scale.has_value() ? *softmax_scale : 1.0 / std::sqrt(double(head_dim));
   const float softcap_log2 = logit_softcap > 0.0 ? float(logit_softcap * kRcpLn2) : 0.0f;
   const int64_t max_blocks = bt.size(1), window = std::clamp<int64_t>(window_size, 0, 0x7fffffff);
+  const int max_q = int(std::clamp<int64_t>(max_query_len, 0, 0x7fffffff));
+  const int splits = int(std::min<int64_t>(num_kv_splits, 0x7fffffff));
   const int64_t n = fxpr_attention_mx4_plan(int(num_requests), num_tokens, int(num_heads), int(num_kv_heads),
-                                            int(head_dim), int(page_size), int(max_query_len), int(max_blocks),
-                                            int(window), int(int_bits), int(num_kv_splits), nullptr);
+                                            int(head_dim), int(page_size), max_q, int(max_blocks),
+                                            int(window), int(int_bits), splits, nullptr);
   Tensor ws = n > 0 ? bytes(n, q) : Tensor();
   check_rc(fxpr_unified_attention_mx4(
                q.const_data_ptr(), codes.const_data_ptr(), scales.const_data_ptr(), out.mutable_data_ptr(), code_of(t),
                qsl.const_data_ptr<int32_t>(), sl.const_data_ptr<int32_t>(), bt.const_data_ptr<int32_t>(),
                has_alibi ? alibi.const_data_ptr<float>() : nullptr, int(num_requests), num_tokens, int(num_heads),
-               int(num_kv_heads), int(head_dim), int(page_size), int(max_query_len), int(max_blocks), num_blocks,
+               int(num_kv_heads), int(head_dim), int(page_size), max_q, int(max_blocks), num_blocks,
                q.stride(0), q.stride(1), codes.stride(0), codes.stride(1), codes.stride(2), codes.stride(3),
                scales.stride(0), scales.stride(1), scales.stride(2), scales.stride(3), out.stride(0), out.stride(1),
                bt.stride(0), is_causal ? 1 : 0, float(scale * kRcpLn2), softcap_log2, int(window), int(int_bits),
-               int(frac_bits), int(num_kv_splits), n > 0 ? ws.mutable_data_ptr() : nullptr, n, stream_of(q)),
+               int(frac_bits), splits, n > 0 ? ws.mutable_data_ptr() : nullptr, n, stream_of(q)),
            "fxpr_unified_attention_mx4");
   if (!out.is_same(o)) o.copy_(out);
 }

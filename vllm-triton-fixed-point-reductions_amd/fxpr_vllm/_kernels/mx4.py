@@ -55,6 +55,8 @@ def _check_cache(what: str, codes: torch.Tensor, scales: torch.Tensor) -> None:
         raise ValueError(f"{what}: kv_scales must be (num_blocks, 2, block_size, num_kv_heads, head_size / 32)")
     if codes.stride(4) != 1 or scales.stride(4) != 1:
         raise ValueError(f"{what}: kv_codes and kv_scales must be contiguous along a row")
+    if max(codes.shape[2:4]) > 1 << 30:
+        raise ValueError(f"{what}: block_size and num_kv_heads must be at most 2^30")
 
 
 def _same_device(what: str, first: torch.Tensor, *others: torch.Tensor) -> None:
@@ -190,7 +192,8 @@ def unified_attention_run(
     if block_table.numel() % num_requests or (block_table.dim() == 2 and block_table.shape[0] < num_requests):
         raise ValueError("block_table must have a row per request")
     q = _rows(q)
-    out = o if o.stride(2) == 1 else torch.empty_like(o, memory_format=torch.contiguous_format)
+    # (rows of no request stay as they are)
+    out = o if o.stride(2) == 1 else o.clone(memory_format=torch.contiguous_format)
     bt = block_table if block_table.dim() == 2 else block_table.reshape(num_requests, -1)
     if bt.stride(1) != 1:
         bt = bt.contiguous()
@@ -198,20 +201,21 @@ def unified_attention_run(
     alibi = alibi_slopes.contiguous() if has_alibi else None
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(head_dim)
     softcap = float(logit_softcap) * _RCP_LN2 if float(logit_softcap) > 0.0 else 0.0
-    window = min(max(0, int(window_size)), 0x7FFFFFFF)
+    window, max_query_len = (min(max(0, int(x)), 0x7FFFFFFF) for x in (window_size, max_query_len))
+    num_kv_splits = min(num_kv_splits, 0x7FFFFFFF)
     lib = _hip.load()
     with torch.cuda.device(q.device):
         n = lib.fxpr_attention_mx4_plan(num_requests, num_tokens, num_heads, num_kv_heads, head_dim, page_size,
-                                        int(max_query_len), bt.shape[1], window, int(fxp_int_bits), int(num_kv_splits),
+                                        max_query_len, bt.shape[1], window, int(fxp_int_bits), num_kv_splits,
                                         None)
         ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n > 0 else None
         _hip.call(
             "fxpr_unified_attention_mx4", q.data_ptr(), kv_codes.data_ptr(), kv_scales.data_ptr(), out.data_ptr(),
             _hip.DTYPE_CODE[q.dtype], qsl.data_ptr(), sl.data_ptr(), bt.data_ptr(), _hip.ptr(alibi), num_requests,
-            num_tokens, num_heads, num_kv_heads, head_dim, page_size, int(max_query_len), bt.shape[1], num_blocks,
+            num_tokens, num_heads, num_kv_heads, head_dim, page_size, max_query_len, bt.shape[1], num_blocks,
             q.stride(0), q.stride(1), *kv_codes.stride()[:4], *kv_scales.stride()[:4], out.stride(0), out.stride(1),
             bt.stride(0), int(bool(is_causal)), float(scale) * _RCP_LN2, softcap, window, int(fxp_int_bits),
-            int(fxp_frac_bits), int(num_kv_splits), _hip.ptr(ws), n, _hip.stream_ptr(q.device),
+            int(fxp_frac_bits), num_kv_splits, _hip.ptr(ws), n, _hip.stream_ptr(q.device),
         )
     if out is not o:
         o.copy_(out)
