@@ -376,6 +376,24 @@ def test_attention_formats(ib, fb, d):
         b.check(b.run(ib=ib, fb=fb), fb=fb)
 
 
+@pytest.mark.parametrize("opts", [dict(), dict(softcap=3.0), dict(alibi=True), dict(scale=-0.2), dict(window=600, softcap=9.0)],
+                         ids=lambda o: "_".join(f"{k}{v}" for k, v in o.items()) or "plain")
+@pytest.mark.parametrize("ib,fb", [(16, 8), (32, 16), (32, 32), (64, 16)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_few_rows_a_request(d, ib, fb, opts):
+    # workgroups of up to 4, 8 and 16 rows, split and not, under each form of the scores and sums
+    opts = dict(opts)
+    if opts.pop("alibi", False):
+        opts["slopes"] = torch.tensor([2.0 ** -(i + 1) for i in range(8)])
+    for reqs in ([(1, 1100), (1, 513), (1, 40)], [(1, 700), (2, 1300), (2, 64)], [(4, 64), (1, 1100), (3, 600), (7, 90)],
+                 [(4, 64), (7, 600), (50, 700)]):
+        b = Batch(reqs, 8, 2, d, 16, BF if fb != 32 else HF, seed=d + ib)
+        want = b.over_floats(ib=ib, fb=fb, **opts)
+        for splits in (0, 1, 2):
+            for _ in range(2):
+                assert torch.equal(b.run(splits, ib=ib, fb=fb, **opts), want), (reqs, splits)
+
+
 def test_rows_do_not_depend_on_the_batch():
     # a token's output: alone as a decode step, inside a prompt, beside other requests, at any max_query_len
     b = Batch([(90, 600), (1, 40), (3, 1300)], 8, 2, 128, 16, BF, seed=2)

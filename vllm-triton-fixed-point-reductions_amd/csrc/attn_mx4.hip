@@ -58,7 +58,10 @@ Planned plan_mx4(int num_requests, int64_t num_tokens, int num_heads, int num_kv
   if (requested >= 1) {
     s16 = sp = std::min<int64_t>({int64_t(requested), slots, kMaxGridZ});
   } else {
-    const bool only_long = r.p.prompt && num_tokens == int64_t(num_requests) * max_query_len;
+    // (the tokens that the shortest request has when all others have the most: no
+    // split, so no combine launch, for a request of a few rows that is not there)
+    const bool only_long =
+        r.p.prompt && (num_tokens - int64_t(num_requests - 1) * max_query_len) * group >= kPrefillRows;
     if (wgs16 <= (chunks < 4 ? 128 : window > 0 ? 384 : 1024) && !only_long)
       s16 = std::min(chunks, std::clamp<int64_t>(6144 / wgs16, 12, 128));
     if (r.p.prompt && wgsp < 512) sp = std::min(cdiv(512, wgsp), chunks);

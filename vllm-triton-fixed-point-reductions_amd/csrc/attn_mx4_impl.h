@@ -80,6 +80,25 @@ __device__ __forceinline__ int turned(const Mx4Args& m, int x, int pass) {
   return int(v - quotient(v, m.by_reqs) * uint32_t(m.a.num_requests));
 }
 
+// quant() (fxp_device.h) with its saturating conversion in place. The compiler
+// waits for an MFMA result before its own instructions name the result's
+// registers, not before an asm statement does, and an element of a result that
+// nothing reads (a workgroup of few rows) is a free register while the MFMA still
+// writes it; here the register is one that the rounding has just written.
+__device__ __forceinline__ int32_t cvt_sat(float integral) {
+  asm("v_cvt_i32_f32 %0, %0" : "+v"(integral));
+  return __builtin_bit_cast(int32_t, integral);
+}
+template <int BITS> __device__ __forceinline__ int64_t quant(float s) {
+  const float r = __builtin_rintf(s);
+  if constexpr (BITS == 64) {
+    return __builtin_fabsf(r) < 2147483648.0f ? static_cast<int64_t>(cvt_sat(r)) : quant_i64(s);
+  } else {
+    const int32_t v = cvt_sat(r);
+    return BITS == 16 ? (v < -32768 ? -32768 : (v > 32767 ? 32767 : v)) : v;
+  }
+}
+
 // The rounding constant of the fast quantisation: for |x| 2^f < 2^22,
 // fl(x 2^f + 1.5 2^23) (exact product, one rounding, spacing 1, an even
 // constant) has the bits of RNE(x 2^f) + kRound.
