@@ -54,7 +54,8 @@ HERE = Path(__file__).resolve().parent
 sys.path.insert(0, str(HERE))
 from build import COMMON_FLAGS, CSRC, FILE_FLAGS, hipcc  # noqa: E402
 
-DEFAULT_SOURCES = ["gemm_bf16.hip", "gemm_f16.hip", "gemm_f32.hip", "attn_bf16.hip", "attn_f16.hip"]
+DEFAULT_SOURCES = ["attn_mx4_bf16.hip", "attn_mx4_f16.hip", "gemm_bf16.hip", "gemm_f16.hip", "gemm_f32.hip", "attn_bf16.hip",
+                   "attn_f16.hip"]
 KERNELS = re.compile(r"^(_ZN4fxpr\w*(gemm_big_kernel|gemm_f32_kernel|attn_dma_kernel|attn_prefill_dma_kernel|attn_mix_dma_kernel)\w*):")
 ALL_KERNELS = re.compile(r"^(_ZN4fxpr\w+):")
 MFMA_WAIT_STATES = 19
