@@ -339,6 +339,21 @@ def test_prompts_whose_first_and_last_chunks_are_partly_live(m, ctx, window):
             assert torch.equal(b.run(splits, **kw), want), (kw, splits)
 
 
+@pytest.mark.parametrize("opts", [dict(), dict(softcap=3.0), dict(alibi=True), dict(window=3500), dict(causal=False),
+                                  dict(scale=-0.1)], ids=lambda o: "_".join(f"{k}{v}" for k, v in o.items()) or "plain")
+@pytest.mark.parametrize("ib,fb", [(16, 8), (32, 16), (32, 32)])
+@pytest.mark.parametrize("d,dtype", [(64, BF), (128, HF), (128, BF)])
+def test_prompts_over_long_contexts(d, dtype, ib, fb, opts):
+    # enough rows times chunks for workgroups of two row sets, ragged in both
+    opts = dict(opts)
+    if opts.pop("alibi", False):
+        opts["slopes"] = torch.tensor([2.0 ** -(i + 1) for i in range(8)])
+    b = Batch([(500, 5000), (1, 40), (77, 900), (33, 4999)], 8, 2, d, 16, dtype, seed=d)
+    want = b.over_floats(ib=ib, fb=fb, **opts)
+    for splits in (0, 1, 3):
+        assert torch.equal(b.run(splits, ib=ib, fb=fb, **opts), want), splits
+
+
 @pytest.mark.parametrize("d,dtype", [(128, HF), (256, BF)])
 def test_one_prompt_beside_many_decode_steps(d, dtype):
     # requests x the longest one's row tiles are mostly empty: the grid follows the tokens instead

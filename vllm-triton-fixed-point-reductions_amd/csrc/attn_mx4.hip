@@ -37,11 +37,17 @@ struct Planned {
 // workgroups (the last where equal lengths gain: 48 requests of 4000 keys 51 us,
 // unsplit 58; 83 requests under a window of 1024, f16, head size 64: 26.2 us,
 // unsplit 24.0).
-// The prompts' workgroups (128 rows) split while fewer than two fall to a CU,
-// and up to that: 512 new tokens over 4096 keys 94 us with 4 splits, 205 unsplit,
-// 97 with 8; 128 over 16000 97 us with 16, 788 unsplit; 4 x 256 over 4096 180 us
-// with 2, 209 unsplit; with 512 workgroups, 2048 over 4096, 249 us unsplit, 292
-// with 2.
+// The prompts' workgroups take two row sets (128 rows) where a launch has two for
+// every CU, or so many chunks that splits make it about one; smaller launches
+// end sooner with one (512 new tokens alone 23.5 us, with two 32; 128 over 2048
+// keys 30 against 38, over 4096 39 against 41, over 8192 64 against 56; 2 x 512
+// over 2048 93 against 106, 512 over 2048 69 against 62).
+// They split while fewer than two fall to a CU, and up to that: 512 new tokens
+// over 4096 keys 94 us with 4 splits, 205 unsplit, 97 with 8; 128 over 16000 97 us
+// with 16, 788 unsplit; 4 x 256 over 4096 180 us with 2, 209 unsplit; with 512
+// workgroups, 2048 over 4096, 249 us unsplit, 292 with 2. Of two or three chunks
+// only up to 128 workgroups (128 over 1000 keys 29 us, unsplit 40; 8 x 64 over
+// 1000 46 against 41).
 Planned plan_mx4(int num_requests, int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim, int page_size,
                  int max_query_len, int max_blocks, int window, int int_bits, int requested) {
   Planned r;
@@ -51,9 +57,13 @@ Planned plan_mx4(int num_requests, int64_t num_tokens, int num_heads, int num_kv
   r.p.prompt = max_rows >= kPrefillRows;
   const int64_t qtiles = std::min<int64_t>(cdiv(max_rows, QROWS), r.p.prompt ? kShortTiles : int64_t(1) << 40);
   const int64_t wgs16 = int64_t(num_requests) * num_kv_heads * qtiles;
-  const int64_t wgsp = std::max<int64_t>(cdiv(num_tokens * num_heads, row_sets(int_bits, head_dim) * PQROWS), 1);
   // chunks that a row's keys can touch
   const int64_t chunks = window > 0 ? std::min(slots, cdiv(int64_t(window) + max_query_len, TILE * CT) + 1) : slots;
+  auto prompt_wgs = [&](int sets) { return std::max<int64_t>(cdiv(num_tokens * num_heads, int64_t(sets) * PQROWS), 1); };
+  r.p.sets = row_sets(int_bits, head_dim);
+  const int64_t wgs2 = prompt_wgs(2);
+  if (wgs2 < 512 && (chunks < 4 || wgs2 * chunks < 256 || (chunks == 4 && wgs2 >= 256))) r.p.sets = 1;
+  const int64_t wgsp = prompt_wgs(r.p.sets);
   int64_t s16 = 1, sp = 1;
   if (requested >= 1) {
     s16 = sp = std::min<int64_t>({int64_t(requested), slots, kMaxGridZ});
@@ -64,7 +74,7 @@ Planned plan_mx4(int num_requests, int64_t num_tokens, int num_heads, int num_kv
         r.p.prompt && (num_tokens - int64_t(num_requests - 1) * max_query_len) * group >= kPrefillRows;
     if (wgs16 <= (chunks < 4 ? 128 : window > 0 ? 384 : 1024) && !only_long)
       s16 = std::min(chunks, std::clamp<int64_t>(6144 / wgs16, 12, 128));
-    if (r.p.prompt && wgsp < 512) sp = std::min(cdiv(512, wgsp), chunks);
+    if (r.p.prompt && wgsp < (chunks < 4 ? 129 : 512)) sp = std::min(cdiv(512, wgsp), chunks);
   }
   auto layout = [&](int64_t rows) { return ws_layout(rows, num_heads, head_dim, int_bits, true, slots); };
   if (sp > 1 || (s16 > 1 && !r.p.prompt)) {

@@ -118,6 +118,7 @@ struct Mx4Plan {
   int splits = 1;            // key splits of the 16-row workgroups (every splits-th chunk)
   int pq_splits = 1;         // of the prompts' workgroups (chunks dealt evenly)
   bool prompt = false;       // requests of kPrefillRows rows or more in the prompts' workgroups
+  int sets = 1;              // row sets of the prompts' workgroups (at most row_sets())
   int tok_cap = 0;           // AttnArgs::tok_cap
 };
 
@@ -1455,9 +1456,9 @@ template <int BITS> bool fast_of(const AttnArgs& a) {
   return BITS != 64 && a.fxp_scale <= (BITS == 16 ? 16384.0f : 4194304.0f) && !a.alibi && a.scale_log2 > 0.0f;
 }
 
-template <int DT, int BITS, int D, bool SPLIT, bool FAST, bool CAP>
+template <int DT, int BITS, int D, int RS, bool SPLIT, bool FAST, bool CAP>
 int launch_prompt(const Mx4Args& m, dim3 grid, hipStream_t st) {
-  auto kern = attn_mx4_prompt_kernel<DT, BITS, D, SPLIT, FAST, CAP, row_sets(BITS, D)>;
+  auto kern = attn_mx4_prompt_kernel<DT, BITS, D, SPLIT, FAST, CAP, RS>;
   constexpr int lds = 2 * PromptLds<D>::TILEB;
   if constexpr (lds > 64 * 1024) {
     static bool done[64] = {};  // by device (benign race: the attribute is idempotent)
@@ -1474,13 +1475,20 @@ int launch_prompt(const Mx4Args& m, dim3 grid, hipStream_t st) {
   return 0;
 }
 
-template <int DT, int BITS, int D, bool SPLIT> int launch_prompt(const Mx4Args& m, dim3 grid, hipStream_t st) {
+template <int DT, int BITS, int D, int RS, bool SPLIT> int launch_prompt(const Mx4Args& m, dim3 grid, hipStream_t st) {
   if constexpr (BITS != 64) {
     if (fast_of<BITS>(m.a))
-      return m.a.softcap_log2 > 0.0f ? launch_prompt<DT, BITS, D, SPLIT, true, true>(m, grid, st)
-                                     : launch_prompt<DT, BITS, D, SPLIT, true, false>(m, grid, st);
+      return m.a.softcap_log2 > 0.0f ? launch_prompt<DT, BITS, D, RS, SPLIT, true, true>(m, grid, st)
+                                     : launch_prompt<DT, BITS, D, RS, SPLIT, true, false>(m, grid, st);
   }
-  return launch_prompt<DT, BITS, D, SPLIT, false, false>(m, grid, st);
+  return launch_prompt<DT, BITS, D, RS, SPLIT, false, false>(m, grid, st);
+}
+
+template <int DT, int BITS, int D> int launch_prompt(const Mx4Args& m, dim3 grid, bool split, int sets, hipStream_t st) {
+  if constexpr (row_sets(BITS, D) == 2) {
+    if (sets == 2) return split ? launch_prompt<DT, BITS, D, 2, true>(m, grid, st) : launch_prompt<DT, BITS, D, 2, false>(m, grid, st);
+  }
+  return split ? launch_prompt<DT, BITS, D, 1, true>(m, grid, st) : launch_prompt<DT, BITS, D, 1, false>(m, grid, st);
 }
 
 template <int DT, int BITS, int D, bool SPLIT, int MAXE> void launch_rows16(const Mx4Args& m, dim3 grid, hipStream_t st) {
@@ -1510,18 +1518,16 @@ int launch_mx4(Mx4Args m, const Mx4Plan& p, int num_requests, int max_query_len,
   if (p.prompt) {
     a.pq_rows = kPrefillRows;
     qtiles = std::min<int64_t>(qtiles, kShortTiles);
-    constexpr int kRows = row_sets(BITS, D) * PQROWS;
-    const int64_t ptiles = cdiv(max_rows, kRows);
+    const int64_t rows = int64_t(p.sets) * PQROWS, ptiles = cdiv(max_rows, rows);
     // a flat grid over the tokens where requests x the longest one's tiles
     // would be mostly empty
-    const int64_t flat = num_tokens * a.group / kRows + num_requests;
+    const int64_t flat = num_tokens * a.group / rows + num_requests;
     dim3 grid(unsigned(num_requests * a.num_kv_heads), unsigned(ptiles), unsigned(p.pq_splits));
     if (ptiles > 65535 || (num_requests * ptiles - flat) * a.num_kv_heads * p.pq_splits > kFlatEmpty) {
       a.pq_blocks = int(flat);
       grid = dim3(unsigned(flat * a.num_kv_heads), 1, unsigned(p.pq_splits));
     }
-    const int e = p.pq_splits > 1 ? launch_prompt<DT, BITS, D, true>(m, grid, st)
-                                  : launch_prompt<DT, BITS, D, false>(m, grid, st);
+    const int e = launch_prompt<DT, BITS, D>(m, grid, p.pq_splits > 1, p.sets, st);
     if (e) return e;
   }
   const dim3 grid(unsigned(num_requests * a.num_kv_heads), unsigned(qtiles), unsigned(p.splits));
